@@ -117,7 +117,8 @@ int muon_b200_push_copies(void* const* dst, int n, const void* src, int64_t byte
 /* ---- Accounting and per-kernel timing -----------------------------------------------
  * Kernel kinds, in the order of every array below:
  *   0 NS line 1, 1 NS line 2, 2 NS line 3 (work unit: algorithmic FLOPs, symmetric products
- *   counted once), 3 prologue, 4 epilogue, 5 AOL rescale, 6 Frobenius normalise, 7 Adam
+ *   counted once), 3 prologue, 4 epilogue, 5 AOL rescale, 6 Frobenius normalise, 7 Adam,
+ *   8 AdamW (32-bit and 8-bit moments), 9 gradient norm and clipping, 10 moment conversion
  *   (work unit: algorithmic HBM bytes). No counterpart in the reference. */
 int muon_b200_kernel_kinds(void);
 /* Kernel launches issued by this process since load, per kind. */
@@ -342,6 +343,73 @@ int muon_b200_adam(void* const* params, void* const* grads, void* const* exp_avg
                    void* const* exp_avg_sq, const int64_t* numel, const int64_t* steps, int count,
                    int dtype, double lr, double weight_decay, double beta1, double beta2,
                    double eps, muon_b200_stream_t stream);
+
+/* ---- AdamW over many tensors, moments in 32 or in 8 bits ------------------------------------
+ * No counterpart in the reference, whose Adam keeps its moments in the parameter's type and rounds
+ * every intermediate to it (muon_b200_adam). Here all arithmetic is float32:
+ *   g' = g * f;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
+ * and a 16-bit parameter is rounded once, when it is stored.
+ *
+ * Tensors may have any size, 0 included (their pointers may then be null), and any alignment that
+ * their elements have; 16-byte aligned ones are faster. A call takes any number of tensors and issues one launch for several hundred of them.
+ * Scalars (lr, steps, seed ...) are taken when the call is made: a captured call repeats them.
+ * No tensor that is written may overlap another one of the call. */
+
+/* One step on `count` tensors, in place on params, masters, exp_avg and exp_avg_sq. param_dtype:
+ * float32, bfloat16 or float16; grad_dtype: the same, or float32. exp_avg and exp_avg_sq are float32.
+ * masters: NULL, or float32 master weights of 16-bit parameters; the step then reads and updates the
+ * master and stores its rounded copy into the parameter. steps[i] counts from 1. grad_scale: NULL, or
+ * the address on the device of a factor f for every gradient (muon_b200_grad_norm leaves one); when it
+ * is not finite the call changes nothing. */
+int muon_b200_adamw(void* const* params, void* const* masters, void* const* grads, void* const* exp_avg,
+                    void* const* exp_avg_sq, const int64_t* numel, const int64_t* steps, int count,
+                    int param_dtype, int grad_dtype, double lr, double weight_decay, double beta1,
+                    double beta2, double eps, const float* grad_scale, muon_b200_stream_t stream);
+
+/* Moments in 8 bits. A flattened tensor of n elements has n code bytes per moment and
+ * ceil(n / MUON_B200_STATE_BLOCK) float32 scales: one for each block of 256 consecutive elements.
+ *   MUON_B200_EXP_AVG     e4m3 codes (sign, 4 exponent, 3 mantissa bits): value = code * scale,
+ *                         scale = amax / 448, rounded to nearest even
+ *   MUON_B200_EXP_AVG_SQ  codes of 5 exponent and 3 mantissa bits, no sign: code c stands for
+ *                         scale * 2^((c >> 3) - 31) * (1 + (c & 7) / 8), scale = amax / 1.875
+ * amax is the largest magnitude of the block; a block whose amax is under 2^-110 (EXP_AVG) or 2^-120
+ * (EXP_AVG_SQ) gets scale 0. New state is all zeros. muon_b200_adamw8 uses the moments of the step
+ * unrounded for the parameter and rounds them for storage, the second one stochastically: the 20
+ * random bits of an element are a hash of seed, steps[i] and the element's index in its tensor, so a
+ * step can be repeated and does not depend on what else is in the call. eps must be at least 1e-16. A
+ * gradient that is not finite spoils the moments of its block of 256 (grad_scale can keep it out). */
+#define MUON_B200_STATE_BLOCK 256
+#define MUON_B200_EXP_AVG 0
+#define MUON_B200_EXP_AVG_SQ 1
+int muon_b200_adamw8(void* const* params, void* const* masters, void* const* grads,
+                     void* const* exp_avg_codes, void* const* exp_avg_scales,
+                     void* const* exp_avg_sq_codes, void* const* exp_avg_sq_scales, const int64_t* numel,
+                     const int64_t* steps, int count, int param_dtype, int grad_dtype, double lr,
+                     double weight_decay, double beta1, double beta2, double eps, uint32_t seed,
+                     const float* grad_scale, muon_b200_stream_t stream);
+
+/* Values of element type dtype (float32, bfloat16, float16) -> codes and scales (both moments to
+ * nearest; EXP_AVG_SQ expects values that are not negative), and back. */
+int muon_b200_quantize_state(void* const* src, void* const* codes, void* const* scales, const int64_t* numel,
+                             int count, int dtype, int kind, muon_b200_stream_t stream);
+int muon_b200_dequantize_state(void* const* codes, void* const* scales, void* const* dst, const int64_t* numel,
+                               int count, int dtype, int kind, muon_b200_stream_t stream);
+
+/* Norm of all elements of `count` tensors (each with its own element type) and the factor that
+ * brings it down to max_norm, both left on the device: out2[0] = norm, out2[1] = min(1, max_norm /
+ * (norm + 1e-6)), or NaN when the norm is not finite, which makes an AdamW call that reads it change
+ * nothing. The squares of the whole range of float32 are added up without overflow. The order of the
+ * additions depends on the sizes and the device only. scratch: 256-byte aligned, at least
+ * muon_b200_grad_norm_scratch_bytes() bytes, contents irrelevant before and after; not shared with
+ * a call that may run at the same time. */
+int64_t muon_b200_grad_norm_scratch_bytes(void);
+int muon_b200_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                        float* out2, void* scratch, int64_t scratch_bytes, muon_b200_stream_t stream);
+/* The same norm, and every element multiplied by the factor, rounded to its type. out2[1] is the
+ * factor that was applied: 0 for an infinite norm, NaN for one that is not a number. */
+int muon_b200_clip_grads(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                         float* out2, void* scratch, int64_t scratch_bytes, muon_b200_stream_t stream);
 
 #ifdef __cplusplus
 }

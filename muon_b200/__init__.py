@@ -5,6 +5,14 @@ Drop-in for the public names of thib-s/Muon's ``muon`` module. All arithmetic ru
 importing this package fails if that library has not been built.
 """
 from ._lib import MuonB200Error, device_status  # noqa: F401  (import fails loudly without the library)
+from .adamw import (  # noqa: F401
+    adamw8_step,
+    adamw_step,
+    clip_grad_norm_,
+    dequantize_state,
+    grad_norm,
+    quantize_state,
+)
 from .backward_overlap import StepInBackward  # noqa: F401
 from .checkpoint import consolidated_state_dict, load_consolidated_state_dict  # noqa: F401
 from .engine import get_backend, get_ns_mode, mark_grad_ready, set_ns_mode  # noqa: F401
@@ -32,4 +40,5 @@ __all__ = [
     "set_ns_mode", "get_ns_mode", "get_backend", "device_status", "MuonB200Error",
     "mark_grad_ready", "StepInBackward", "consolidated_state_dict", "load_consolidated_state_dict",
     "set_ownership", "get_ownership", "ShardedMuon",
+    "adamw_step", "adamw8_step", "grad_norm", "clip_grad_norm_", "quantize_state", "dequantize_state",
 ]

@@ -7,12 +7,13 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_uint32, c_void_p
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libmuon_b200.so")
 
 F32, BF16, F16, F64 = 0, 1, 2, 3
+EXP_AVG, EXP_AVG_SQ, STATE_BLOCK = 0, 1, 256  # MUON_B200_EXP_AVG, MUON_B200_EXP_AVG_SQ, MUON_B200_STATE_BLOCK
 NS_AOL4, NS_CLASSIC5, NS_AOL4_FP8 = 0, 1, 2
 NS_HAVE_SUMSQ = 0x100  # MUON_B200_NS_HAVE_SUMSQ
 
@@ -104,6 +105,15 @@ PROTOTYPES = {
     "muon_b200_adam": (c_int, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p),
                                POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64), c_int, c_int,
                                c_double, c_double, c_double, c_double, c_double, c_void_p]),
+    # (tables of the calls below are passed as addresses, see address_table)
+    "muon_b200_adamw": (c_int, [c_void_p] * 7 + [c_int, c_int, c_int] + [c_double] * 5 + [c_void_p, c_void_p]),
+    "muon_b200_adamw8": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int] + [c_double] * 5
+                         + [c_uint32, c_void_p, c_void_p]),
+    "muon_b200_quantize_state": (c_int, [c_void_p] * 4 + [c_int, c_int, c_int, c_void_p]),
+    "muon_b200_dequantize_state": (c_int, [c_void_p] * 4 + [c_int, c_int, c_int, c_void_p]),
+    "muon_b200_grad_norm_scratch_bytes": (c_int64, []),
+    "muon_b200_grad_norm": (c_int, [c_void_p] * 3 + [c_int, c_double, c_void_p, c_void_p, c_int64, c_void_p]),
+    "muon_b200_clip_grads": (c_int, [c_void_p] * 3 + [c_int, c_double, c_void_p, c_void_p, c_int64, c_void_p]),
 }
 
 
@@ -136,6 +146,12 @@ def i64_array(vals) -> ctypes.Array:
     return (c_int64 * len(vals))(*vals)
 
 
+def address(table) -> int:
+    """Address of an ``array.array`` (a table of pointers, sizes or steps). The caller keeps the array
+    alive until the call has returned."""
+    return table.buffer_info()[0]
+
+
 def device_status(reset: bool = True) -> int:
     """Synchronises the device and returns the kernels' status word (0 = healthy)."""
     st = c_int(0)
@@ -144,7 +160,7 @@ def device_status(reset: bool = True) -> int:
 
 
 KERNEL_KINDS = ("ns_line1", "ns_line2", "ns_line3", "prologue", "epilogue", "aol_rescale",
-                "fro_normalize", "adam")
+                "fro_normalize", "adam", "adamw", "grad_norm", "state_convert")
 
 
 def launch_counts() -> dict:

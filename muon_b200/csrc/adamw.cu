@@ -1,0 +1,975 @@
+// Multi-tensor AdamW: see adamw.h. All kernels here are bound by HBM traffic.
+#include "adamw.h"
+
+#include "common.cuh"
+#include "elementwise.h"
+#include "ns_gemm.h"
+#include "profiling.h"
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cmath>
+
+namespace mb {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+// ---------------------------------------------------------------------------
+// N consecutive elements of T as floats. N * sizeof(T) is a multiple of 16 bytes.
+// Every element is touched once per call: streaming accesses.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float to_float(T v);
+template <>
+__device__ __forceinline__ float to_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t w, float& a, float& b);
+template <>
+__device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t w, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+template <>
+__device__ __forceinline__ void unpack2<__half>(uint32_t w, float& a, float& b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = f.x;
+  b = f.y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int N>
+struct Raw {  // the words of N elements, as loaded
+  static constexpr int kWords = N * (int)sizeof(T) / 16;
+  uint4 w[kWords];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) __stcs(reinterpret_cast<uint4*>(p) + k, w[k]);
+  }
+  __device__ __forceinline__ void unpack(float (&v)[N]) const {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) v[4 * k + j] = __uint_as_float(u[j]);
+        else unpack2<T>(u[j], v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
+      }
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&v)[N]) {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) u[j] = __float_as_uint(v[4 * k + j]);
+        else u[j] = pack2<T>(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
+      }
+      w[k] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+};
+
+__device__ __forceinline__ float sqrt_approx(float x) {  // relative error at most 2^-23
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Index of the table entry whose range of chunks holds `chunk` (start[0] = 0, ascending).
+template <typename S>
+__device__ __forceinline__ int find_tensor(const S& start, int count, int chunk) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (chunk >= start[mid]) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+struct AdamWConsts {
+  float b1, w1, b2, w2;  // float(beta), float(1 - beta)
+  float eps, decay;      // decay = float(1 - lr * weight_decay)
+  const float* grad_scale;
+  int count;
+};
+
+// p (1 - lr wd) - (lr / c1) m / (sqrt(v) / sqrt(c2) + eps). The square root and the quotient are the
+// hardware's approximations (about 2^-22 together): they only scale an update that is itself a
+// small fraction of p.
+__device__ __forceinline__ float moved(float p, float m, float v, float decay, float step, float rs, float eps) {
+  const float den = fmaf(sqrt_approx(v), rs, eps);
+  return fmaf(-step, __fdividef(m, den), p * decay);
+}
+
+// The factor that every gradient is multiplied by. A factor that is not finite (the norm was not)
+// means: leave everything as it is.
+__device__ __forceinline__ bool read_factor(const float* grad_scale, float& f) {
+  f = grad_scale ? __ldg(grad_scale) : 1.f;
+  return fabsf(f) <= 3.402823466e38f;
+}
+
+// ---------------------------------------------------------------------------
+// AdamW with 32-bit moments.
+//   g' = g f;  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2
+//   p  = p (1 - lr wd) - (lr/c1) m / (sqrt(v)/sqrt(c2) + eps)
+// in float32 registers, p rounded once when it is stored. With a master weight p is the master and
+// the parameter receives its rounded copy.
+// ---------------------------------------------------------------------------
+template <int CAP>
+struct AdamW32Args {
+  AdamWConsts c;
+  void* p[CAP];
+  float* w[CAP];
+  const void* g[CAP];
+  float* m[CAP];
+  float* v[CAP];
+  long long numel[CAP];
+  float step[CAP], rs[CAP];
+  int start[CAP + 1];
+  unsigned char vec_ok[CAP];
+};
+
+template <typename P>
+constexpr int kVec32 = sizeof(P) == 4 ? 4 : 8;
+constexpr int kIters32 = 4;
+template <typename P>
+constexpr int kChunk32 = kThreads * kVec32<P> * kIters32;
+
+template <typename P, typename G, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kThreads)
+adamw32_kernel(const __grid_constant__ AdamW32Args<CAP> a) {
+  constexpr int V = kVec32<P>;
+  float f;
+  if (!read_factor(a.c.grad_scale, f)) return;
+  const int t = find_tensor(a.start, a.c.count, (int)blockIdx.x);
+  const long long base = (long long)((int)blockIdx.x - a.start[t]) * kChunk32<P>;
+  const long long left = a.numel[t] - base;
+  P* p = static_cast<P*>(a.p[t]) + base;
+  float* w = MASTER ? a.w[t] + base : nullptr;
+  const G* g = static_cast<const G*>(a.g[t]) + base;
+  float* m = a.m[t] + base;
+  float* v = a.v[t] + base;
+  const float step = a.step[t], rs = a.rs[t];
+  const AdamWConsts c = a.c;
+  const auto one = [&](float& pj, float gj, float& mj, float& vj) {
+    gj *= f;
+    mj = fmaf(gj, c.w1, mj * c.b1);
+    vj = fmaf(gj * gj, c.w2, vj * c.b2);
+    pj = moved(pj, mj, vj, c.decay, step, rs, c.eps);
+  };
+  int done = 0;  // elements of the chunk that the vector loop covers
+  if (a.vec_ok[t]) {
+    done = left >= kChunk32<P> ? kChunk32<P> : (int)left / V * V;
+#pragma unroll 2
+    for (int i = threadIdx.x * V; i < done; i += kThreads * V) {
+      Raw<P, V> rp;
+      Raw<float, V> rw, rm, rv;
+      Raw<G, V> rg;
+      if constexpr (MASTER) rw.load(w + i);
+      else rp.load(p + i);
+      rg.load(g + i);
+      rm.load(m + i);
+      rv.load(v + i);
+      float pj[V], gj[V], mj[V], vj[V];
+      if constexpr (MASTER) rw.unpack(pj);
+      else rp.unpack(pj);
+      rg.unpack(gj);
+      rm.unpack(mj);
+      rv.unpack(vj);
+#pragma unroll
+      for (int j = 0; j < V; ++j) one(pj[j], gj[j], mj[j], vj[j]);
+      rm.pack(mj);
+      rm.store(m + i);
+      rv.pack(vj);
+      rv.store(v + i);
+      if constexpr (MASTER) {
+        rw.pack(pj);
+        rw.store(w + i);
+      }
+      rp.pack(pj);
+      rp.store(p + i);
+    }
+  }
+  const int end = left < kChunk32<P> ? (int)left : kChunk32<P>;
+  for (int i = done + threadIdx.x; i < end; i += kThreads) {
+    float pj = MASTER ? w[i] : to_float<P>(p[i]), mj = m[i], vj = v[i];
+    one(pj, to_float<G>(g[i]), mj, vj);
+    m[i] = mj;
+    v[i] = vj;
+    if (MASTER) w[i] = pj;
+    p[i] = from_float<P>(pj);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit moments. A block of kStateBlock consecutive elements shares a float32 scale per moment; one
+// warp handles a block, eight elements a lane.
+//   first moment   e4m3, value = code * scale, scale = amax / 448, nearest even
+//   second moment  5 exponent and 3 mantissa bits without a sign: value = scale * w(c), where w(c) is the
+//                  float whose bits are (c + 768) << 20, i.e. 2^((c >> 3) - 31) (1 + (c & 7) / 8);
+//                  scale = amax / 1.875 = amax / w(255)
+// Neither needs a table. Unsigned: a second moment has no sign, so its mantissa gets that bit; 32
+// binades hold gradients that differ by 2^16 within a block; code 0 stands for 2^-31, so no element of a
+// block that is in use ever divides by nothing.
+//
+// What is rounded to a code, and the code, are a function of float32 operations with one rounding each
+// (no fused multiply-add): the same step written in any float32 arithmetic gives the same codes.
+//
+// The second moment is rounded stochastically in a step: with beta2 = 0.999 a step moves it by a
+// thousandth, a code is 6 to 12 percent wide, and rounding to nearest would never move it.
+// x = v * (1.875 / amax) as bits, plus 20 random bits, cut at bit 20: right on average, exactly.
+// ---------------------------------------------------------------------------
+constexpr float kE4m3Max = 448.f, kSqMax = 1.875f;
+constexpr float kTinyAvg = 0x1p-110f, kTinySq = 0x1p-120f;  // below: the block counts as zero
+
+template <int KIND>
+__device__ __forceinline__ void block_scale(float amax, float& scale, float& inv) {
+  constexpr float top = KIND == STATE_EXP_AVG ? kE4m3Max : kSqMax;
+  const bool tiny = amax < (KIND == STATE_EXP_AVG ? kTinyAvg : kTinySq);
+  scale = tiny ? 0.f : __fmul_rn(amax, 1.f / top);
+  inv = tiny ? 0.f : __fdiv_rn(top, amax);
+}
+
+// Largest |x| of a warp's eight elements a lane, by the bits: a NaN is above everything.
+__device__ __forceinline__ float warp_amax(const float (&x)[8]) {
+  uint32_t b = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b = max(b, __float_as_uint(x[j]) & 0x7fffffffu);
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, b));
+}
+
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3_values(uint32_t pair) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ float sq_value(uint32_t code) { return __uint_as_float((code + 768u) << 20); }
+__device__ __forceinline__ uint32_t sq_code(float x, uint32_t r) {
+  const int c = ((int)(__float_as_uint(x) + r) >> 20) - 768;
+  return (uint32_t)min(max(c, 0), 255);
+}
+
+// Eight codes of a moment <-> floats.
+template <int KIND>
+__device__ __forceinline__ void decode8(uint2 w, float scale, float (&x)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t u = h ? w.y : w.x;
+    if constexpr (KIND == STATE_EXP_AVG) {
+      const float2 lo = e4m3_values(u & 0xffffu), hi = e4m3_values(u >> 16);
+      x[4 * h] = lo.x; x[4 * h + 1] = lo.y; x[4 * h + 2] = hi.x; x[4 * h + 3] = hi.y;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * h + j] = sq_value((u >> (8 * j)) & 0xffu);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], scale);
+}
+template <int KIND>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv, const uint32_t (&r)[8]) {
+  uint32_t u[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(x[4 * h + j], inv);
+    if constexpr (KIND == STATE_EXP_AVG) {
+      u[h] = e4m3_pair(y[0], y[1]) | e4m3_pair(y[2], y[3]) << 16;
+      if (inv == 0.f) u[h] = y[0] == y[0] ? 0u : u[h];
+    } else {
+      u[h] = sq_code(y[0], r[4 * h]) | sq_code(y[1], r[4 * h + 1]) << 8 | sq_code(y[2], r[4 * h + 2]) << 16 |
+             sq_code(y[3], r[4 * h + 3]) << 24;
+    }
+  }
+  return make_uint2(u[0], u[1]);
+}
+
+// 32 random bits for the four elements 4 * word .. 4 * word + 3; element j takes the low 20 bits of
+// the word turned right by 8 j. The multipliers are the fractional parts of the golden ratio and of
+// the square roots of 2 and 3.
+__device__ __forceinline__ uint32_t random_word(uint32_t word, uint32_t key) {
+  uint32_t h = word * 0x9E3779B1u + key;
+  h = (h ^ (h >> 16)) * 0x6A09E667u;
+  h = (h ^ (h >> 15)) * 0xBB67AE85u;
+  return h ^ (h >> 16);
+}
+__device__ __forceinline__ uint32_t random_bits(uint32_t h, int j) { return __funnelshift_r(h, h, 8 * j) & 0xfffffu; }
+inline uint32_t random_key(uint32_t seed, int64_t step) { return seed * 0x3C6EF373u + (uint32_t)step * 0xBB67AE85u; }
+
+template <int CAP>
+struct AdamW8Args {
+  AdamWConsts c;
+  void* p[CAP];
+  float* w[CAP];
+  const void* g[CAP];
+  uint8_t* m[CAP];
+  float* ms[CAP];
+  uint8_t* v[CAP];
+  float* vs[CAP];
+  long long numel[CAP];
+  float step[CAP], rs[CAP];
+  uint32_t key[CAP];
+  int start[CAP + 1];
+  unsigned char vec_ok[CAP];
+};
+
+constexpr int kBlocksPerWarp = 4;
+constexpr int kBlocksPerChunk = kWarps * kBlocksPerWarp;
+
+template <typename P, typename G, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kThreads)
+adamw8_kernel(const __grid_constant__ AdamW8Args<CAP> a) {
+  float f;
+  if (!read_factor(a.c.grad_scale, f)) return;
+  const int t = find_tensor(a.start, a.c.count, (int)blockIdx.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long numel = a.numel[t];
+  const long long blocks = (numel + kStateBlock - 1) / kStateBlock;
+  P* p = static_cast<P*>(a.p[t]);
+  float* w = MASTER ? a.w[t] : nullptr;
+  const G* g = static_cast<const G*>(a.g[t]);
+  uint8_t *m = a.m[t], *v = a.v[t];
+  const float step = a.step[t], rs = a.rs[t];
+  const uint32_t key = a.key[t];
+  const AdamWConsts c = a.c;
+  const long long first = (long long)((int)blockIdx.x - a.start[t]) * kBlocksPerChunk + warp;
+  for (int k = 0; k < kBlocksPerWarp; ++k) {
+    const long long b = first + (long long)k * kWarps;
+    if (b >= blocks) return;
+    const long long base = b * kStateBlock;
+    const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
+    const float ms = a.ms[t][b], vs = a.vs[t][b];
+    float pj[8], gj[8], mj[8], vj[8];
+    uint32_t r[8];
+    const long long at = base + lane * 8;  // this lane's elements: eight in a row, or every 32nd
+    if (vec) {
+      Raw<G, 8> rg;
+      rg.load(g + at);
+      if constexpr (MASTER) {
+        Raw<float, 8> rw;
+        rw.load(w + at);
+        rw.unpack(pj);
+      } else {
+        Raw<P, 8> rp;
+        rp.load(p + at);
+        rp.unpack(pj);
+      }
+      const uint2 cm = __ldcs(reinterpret_cast<const uint2*>(m + at));
+      const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(v + at));
+      rg.unpack(gj);
+      decode8<STATE_EXP_AVG>(cm, ms, mj);
+      decode8<STATE_EXP_AVG_SQ>(cv, vs, vj);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t bits = random_word((uint32_t)(at >> 2) + h, key);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[4 * h + j] = random_bits(bits, j);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const long long i = base + lane + 32 * j;
+        const bool in = i < numel;
+        pj[j] = in ? (MASTER ? w[i] : to_float<P>(p[i])) : 0.f;
+        gj[j] = in ? to_float<G>(g[i]) : 0.f;
+        mj[j] = in ? __fmul_rn(e4m3_values(m[i]).x, ms) : 0.f;
+        vj[j] = in ? __fmul_rn(sq_value(v[i]), vs) : 0.f;
+        r[j] = random_bits(random_word((uint32_t)(i >> 2), key), (int)(i & 3));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      gj[j] = __fmul_rn(gj[j], f);
+      mj[j] = __fadd_rn(__fmul_rn(mj[j], c.b1), __fmul_rn(gj[j], c.w1));
+      vj[j] = __fadd_rn(__fmul_rn(vj[j], c.b2), __fmul_rn(__fmul_rn(gj[j], gj[j]), c.w2));
+      pj[j] = moved(pj[j], mj[j], vj[j], c.decay, step, rs, c.eps);
+    }
+    float m_scale, m_inv, v_scale, v_inv;
+    block_scale<STATE_EXP_AVG>(warp_amax(mj), m_scale, m_inv);
+    block_scale<STATE_EXP_AVG_SQ>(warp_amax(vj), v_scale, v_inv);
+    if (lane == 0) {
+      a.ms[t][b] = m_scale;
+      a.vs[t][b] = v_scale;
+    }
+    const uint2 cm = encode8<STATE_EXP_AVG>(mj, m_inv, r);
+    const uint2 cv = encode8<STATE_EXP_AVG_SQ>(vj, v_inv, r);
+    if (vec) {
+      __stcs(reinterpret_cast<uint2*>(m + at), cm);
+      __stcs(reinterpret_cast<uint2*>(v + at), cv);
+      if constexpr (MASTER) {
+        Raw<float, 8> rw;
+        rw.pack(pj);
+        rw.store(w + at);
+      }
+      Raw<P, 8> rp;
+      rp.pack(pj);
+      rp.store(p + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const long long i = base + lane + 32 * j;
+        if (i < numel) {
+          m[i] = (uint8_t)((j < 4 ? cm.x : cm.y) >> (8 * (j & 3)));
+          v[i] = (uint8_t)((j < 4 ? cv.x : cv.y) >> (8 * (j & 3)));
+          if (MASTER) w[i] = pj[j];
+          p[i] = from_float<P>(pj[j]);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Conversion of moments: 32-bit (or 16-bit) values <-> codes and scales.
+// ---------------------------------------------------------------------------
+template <int CAP>
+struct ConvertArgs {
+  void* x[CAP];
+  uint8_t* codes[CAP];
+  float* scales[CAP];
+  long long numel[CAP];
+  int start[CAP + 1];
+  unsigned char vec_ok[CAP];
+  int count;
+};
+
+template <typename T, int KIND, bool TO_CODES, int CAP>
+__global__ void __launch_bounds__(kThreads)
+convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
+  const int t = find_tensor(a.start, a.count, (int)blockIdx.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long numel = a.numel[t];
+  const long long blocks = (numel + kStateBlock - 1) / kStateBlock;
+  T* x = static_cast<T*>(a.x[t]);
+  uint8_t* codes = a.codes[t];
+  float* scales = a.scales[t];
+  const long long first = (long long)((int)blockIdx.x - a.start[t]) * kBlocksPerChunk + warp;
+#pragma unroll
+  for (int k = 0; k < kBlocksPerWarp; ++k) {
+    const long long b = first + (long long)k * kWarps;
+    if (b >= blocks) return;
+    const long long base = b * kStateBlock;
+    const long long at = base + lane * 8;
+    const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
+    float xj[8];
+    if constexpr (TO_CODES) {
+      if (vec) {
+        Raw<T, 8> rx;
+        rx.load(x + at);
+        rx.unpack(xj);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const long long i = base + lane + 32 * j;
+          xj[j] = i < numel ? to_float<T>(x[i]) : 0.f;
+        }
+      }
+      float scale, inv;
+      block_scale<KIND>(warp_amax(xj), scale, inv);
+      if (lane == 0) scales[b] = scale;
+      const uint32_t half = 1u << 19;  // nearest: half a code is added before the cut
+      const uint32_t r[8] = {half, half, half, half, half, half, half, half};
+      const uint2 c = encode8<KIND>(xj, inv, r);
+      if (vec) {
+        __stcs(reinterpret_cast<uint2*>(codes + at), c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const long long i = base + lane + 32 * j;
+          if (i < numel) codes[i] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+        }
+      }
+    } else {
+      const float scale = scales[b];
+      if (vec) {
+        decode8<KIND>(__ldcs(reinterpret_cast<const uint2*>(codes + at)), scale, xj);
+        Raw<T, 8> rx;
+        rx.pack(xj);
+        rx.store(x + at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const long long i = base + lane + 32 * j;
+          if (i < numel) {
+            const uint32_t c = codes[i];
+            x[i] = from_float<T>(__fmul_rn(KIND == STATE_EXP_AVG ? e4m3_values(c).x : sq_value(c), scale));
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Global gradient norm. Squares are added in float32 over eight elements and in float64 from there on,
+// in an order that depends on the sizes alone. Where the eight squares overflow, or are so small that
+// they lose bits, the eight are squared in float64 instead: the norm is right over the whole range of
+// the type.
+// ---------------------------------------------------------------------------
+template <int CAP>
+struct NormArgs {
+  void* x[CAP];
+  long long numel[CAP];
+  int start[CAP + 1];
+  unsigned char dtype[CAP];
+  unsigned char vec_ok[CAP];
+  int count, chunks;
+  double* partials;
+};
+
+constexpr int kNormIters = 4;
+constexpr int kNormChunk = kThreads * 8 * kNormIters;
+
+__device__ __forceinline__ double squares(const float (&x)[8]) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], s);
+  if (s < 3e38f && s > 1e-30f) return (double)s;
+  uint32_t any = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) any |= __float_as_uint(x[j]) << 1;
+  if (any == 0) return 0.0;
+  double d = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d += (double)x[j] * (double)x[j];
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ double chunk_squares(const T* x, long long left, bool vec) {
+  double acc = 0.0;
+  int done = 0;
+  const int end = left < kNormChunk ? (int)left : kNormChunk;
+  if (vec) {
+    done = end / 8 * 8;
+#pragma unroll
+    for (int k = 0; k < kNormIters; ++k) {
+      const int i = (k * kThreads + threadIdx.x) * 8;
+      if (i < done) {
+        Raw<T, 8> rx;
+        rx.load(x + i);
+        float v[8];
+        rx.unpack(v);
+        acc += squares(v);
+      }
+    }
+  }
+  for (int i = done + threadIdx.x; i < end; i += kThreads) {
+    const double v = (double)to_float<T>(x[i]);
+    acc += v * v;
+  }
+  return acc;
+}
+
+// Sum over the block, to every thread; the order of the additions is fixed.
+__device__ __forceinline__ double block_sum(double v, double (&warps)[kWarps]) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < kWarps; ++k) s += warps[k];
+  return s;
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kThreads)
+norm_partial_kernel(const __grid_constant__ NormArgs<CAP> a) {
+  __shared__ double warps[kWarps];
+  double acc = 0.0;
+  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int t = find_tensor(a.start, a.count, chunk);
+    const long long base = (long long)(chunk - a.start[t]) * kNormChunk;
+    const long long left = a.numel[t] - base;
+    const bool vec = a.vec_ok[t] != 0;
+    if (a.dtype[t] == DT_F32) acc += chunk_squares(static_cast<const float*>(a.x[t]) + base, left, vec);
+    else if (a.dtype[t] == DT_BF16) acc += chunk_squares(static_cast<const __nv_bfloat16*>(a.x[t]) + base, left, vec);
+    else acc += chunk_squares(static_cast<const __half*>(a.x[t]) + base, left, vec);
+  }
+  acc = block_sum(acc, warps);
+  if (threadIdx.x == 0) a.partials[blockIdx.x] = acc;
+}
+
+// {norm, factor} from the partial sums: every block that needs them adds them up in the same order.
+__device__ __forceinline__ float2 finish_norm(const double* partials, int n, float max_norm, double (&warps)[kWarps]) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) acc += partials[i];
+  const float norm = (float)sqrt(block_sum(acc, warps));
+  const float q = max_norm / (norm + 1e-6f);
+  return make_float2(norm, q > 1.f ? 1.f : q);  // a NaN stays
+}
+
+__global__ void __launch_bounds__(kThreads)
+norm_finish_kernel(const double* partials, int n, float max_norm, float* out2) {
+  __shared__ double warps[kWarps];
+  const float2 r = finish_norm(partials, n, max_norm, warps);
+  if (threadIdx.x == 0) {
+    out2[0] = r.x;
+    out2[1] = fabsf(r.x) <= 3.402823466e38f ? r.y : __int_as_float(0x7fffffff);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_chunk(T* x, long long left, bool vec, float f) {
+  int done = 0;
+  const int end = left < kNormChunk ? (int)left : kNormChunk;
+  if (vec) {
+    done = end / 8 * 8;
+#pragma unroll
+    for (int k = 0; k < kNormIters; ++k) {
+      const int i = (k * kThreads + threadIdx.x) * 8;
+      if (i < done) {
+        Raw<T, 8> rx;
+        rx.load(x + i);
+        float v[8];
+        rx.unpack(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= f;
+        rx.pack(v);
+        rx.store(x + i);
+      }
+    }
+  }
+  for (int i = done + threadIdx.x; i < end; i += kThreads) x[i] = from_float<T>(to_float<T>(x[i]) * f);
+}
+
+template <int CAP>
+__global__ void __launch_bounds__(kThreads)
+clip_kernel(const __grid_constant__ NormArgs<CAP> a, int partials, float max_norm, float* out2) {
+  __shared__ double warps[kWarps];
+  const float2 r = finish_norm(a.partials, partials, max_norm, warps);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    out2[0] = r.x;
+    out2[1] = r.y;
+  }
+  const float f = r.y;
+  if (f == 1.f) return;  // nothing to clip: x * 1 is x
+  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+    const int t = find_tensor(a.start, a.count, chunk);
+    const long long base = (long long)(chunk - a.start[t]) * kNormChunk;
+    const long long left = a.numel[t] - base;
+    const bool vec = a.vec_ok[t] != 0;
+    if (a.dtype[t] == DT_F32) scale_chunk(static_cast<float*>(a.x[t]) + base, left, vec, f);
+    else if (a.dtype[t] == DT_BF16) scale_chunk(static_cast<__nv_bfloat16*>(a.x[t]) + base, left, vec, f);
+    else scale_chunk(static_cast<__half*>(a.x[t]) + base, left, vec, f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side: tables are filled tensor by tensor and launched when full.
+// ---------------------------------------------------------------------------
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline int elem_bytes(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+// Adds `chunks` to the running total of a launch; false when the launch must go out first.
+inline bool fits(int total, int64_t chunks) { return chunks <= (int64_t)INT32_MAX - total; }
+
+template <typename P, typename G, bool MASTER, int CAP>
+int adamw32_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
+  AdamW32Args<CAP> a;
+  a.c = consts;
+  const double bytes = (MASTER ? sizeof(P) + 8.0 : 2.0 * sizeof(P)) + sizeof(G) + 16.0;
+  int n = 0;
+  double elems = 0;
+  a.start[0] = 0;
+  for (int i = 0; i <= c.count; ++i) {
+    const int64_t chunks = i < c.count ? (c.numel[i] + kChunk32<P> - 1) / kChunk32<P> : 0;
+    if (i == c.count || n == CAP || !fits(a.start[n], chunks)) {
+      if (n > 0) {
+        a.c.count = n;
+        LaunchScope scope(K_ADAMW, elems * bytes, stream);
+        adamw32_kernel<P, G, MASTER, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
+        MB_CUDA_CHECK(cudaGetLastError());
+      }
+      n = 0;
+      elems = 0;
+    }
+    if (chunks == 0) continue;
+    a.p[n] = c.param[i];
+    a.w[n] = MASTER ? static_cast<float*>(c.master[i]) : nullptr;
+    a.g[n] = c.grad[i];
+    a.m[n] = static_cast<float*>(c.exp_avg[i]);
+    a.v[n] = static_cast<float*>(c.exp_avg_sq[i]);
+    a.numel[n] = c.numel[i];
+    a.step[n] = (float)(c.lr / (1.0 - std::pow(c.beta1, (double)c.steps[i])));
+    a.rs[n] = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)c.steps[i])));
+    a.vec_ok[n] = aligned(a.p[n], 16) && aligned(a.g[n], 16) && aligned(a.m[n], 16) && aligned(a.v[n], 16) &&
+                  aligned(a.w[n], 16);
+    a.start[n + 1] = a.start[n] + (int)chunks;
+    elems += (double)c.numel[i];
+    ++n;
+  }
+  return OK;
+}
+
+template <typename P, typename G, bool MASTER, int CAP>
+int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
+  AdamW8Args<CAP> a;
+  a.c = consts;
+  const double bytes = (MASTER ? sizeof(P) + 8.0 : 2.0 * sizeof(P)) + sizeof(G) + 4.0 + 16.0 / kStateBlock;
+  int n = 0;
+  double elems = 0;
+  a.start[0] = 0;
+  for (int i = 0; i <= c.count; ++i) {
+    const int64_t per = (int64_t)kBlocksPerChunk * kStateBlock;
+    const int64_t chunks = i < c.count ? (c.numel[i] + per - 1) / per : 0;
+    if (i == c.count || n == CAP || !fits(a.start[n], chunks)) {
+      if (n > 0) {
+        a.c.count = n;
+        LaunchScope scope(K_ADAMW, elems * bytes, stream);
+        adamw8_kernel<P, G, MASTER, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
+        MB_CUDA_CHECK(cudaGetLastError());
+      }
+      n = 0;
+      elems = 0;
+    }
+    if (chunks == 0) continue;
+    a.p[n] = c.param[i];
+    a.w[n] = MASTER ? static_cast<float*>(c.master[i]) : nullptr;
+    a.g[n] = c.grad[i];
+    a.m[n] = static_cast<uint8_t*>(c.exp_avg[i]);
+    a.ms[n] = static_cast<float*>(c.exp_avg_scale[i]);
+    a.v[n] = static_cast<uint8_t*>(c.exp_avg_sq[i]);
+    a.vs[n] = static_cast<float*>(c.exp_avg_sq_scale[i]);
+    a.numel[n] = c.numel[i];
+    a.step[n] = (float)(c.lr / (1.0 - std::pow(c.beta1, (double)c.steps[i])));
+    a.rs[n] = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)c.steps[i])));
+    a.key[n] = random_key(c.seed, c.steps[i]);
+    a.vec_ok[n] = aligned(a.p[n], 16) && aligned(a.g[n], 16) && aligned(a.m[n], 8) && aligned(a.v[n], 8) &&
+                  aligned(a.w[n], 16);
+    a.start[n + 1] = a.start[n] + (int)chunks;
+    elems += (double)c.numel[i];
+    ++n;
+  }
+  return OK;
+}
+
+constexpr int kCapAdamW32 = 512, kCapAdamW8 = 384, kCapConvert = 512, kCapNorm = 1024;
+
+template <typename P, typename G, bool MASTER>
+int adamw_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
+  if (c.exp_avg_scale) return adamw8_launch<P, G, MASTER, kCapAdamW8>(c, consts, stream);
+  return adamw32_launch<P, G, MASTER, kCapAdamW32>(c, consts, stream);
+}
+
+template <typename P, typename G>
+int adamw_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
+  if constexpr (sizeof(P) == 4) return adamw_launch<P, G, false>(c, consts, stream);
+  else return c.master ? adamw_launch<P, G, true>(c, consts, stream) : adamw_launch<P, G, false>(c, consts, stream);
+}
+
+template <int CAP, typename LAUNCH>
+int for_each_norm_table(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double* partials,
+                        LAUNCH launch) {
+  NormArgs<CAP> a;
+  a.partials = partials;
+  int n = 0;
+  double bytes = 0;
+  a.start[0] = 0;
+  for (int i = 0; i <= count; ++i) {
+    const int64_t chunks = i < count ? (numel[i] + kNormChunk - 1) / kNormChunk : 0;
+    if (i == count || n == CAP || !fits(a.start[n], chunks)) {
+      if (n > 0) {
+        a.count = n;
+        a.chunks = a.start[n];
+        const int rc = launch(a, bytes);
+        if (rc != OK) return rc;
+      }
+      n = 0;
+      bytes = 0;
+    }
+    if (chunks == 0) continue;
+    a.x[n] = tensors[i];
+    a.numel[n] = numel[i];
+    a.dtype[n] = (unsigned char)dtypes[i];
+    a.vec_ok[n] = aligned(tensors[i], 16);
+    a.start[n + 1] = a.start[n] + (int)chunks;
+    bytes += (double)numel[i] * elem_bytes(dtypes[i]);
+    ++n;
+  }
+  return OK;
+}
+
+constexpr int kNormBlocksPerSm = 8;
+constexpr int kNormTables = 64;  // launches of the norm kernel per call: 64 * 1024 tensors
+
+int norm_grid(int chunks, int* grid) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  if (rc != OK) return rc;
+  *grid = chunks < sms * kNormBlocksPerSm ? chunks : sms * kNormBlocksPerSm;
+  return OK;
+}
+
+int norm_partials(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double* partials,
+                  int* n_partials, cudaStream_t stream) {
+  int used = 0, tables = 0;
+  const int rc = for_each_norm_table<kCapNorm>(
+      tensors, numel, dtypes, count, partials, [&](NormArgs<kCapNorm>& a, double bytes) -> int {
+        int grid = 0;
+        const int rc = norm_grid(a.chunks, &grid);
+        if (rc != OK) return rc;
+        if (++tables > kNormTables) return set_error(ERR_UNSUPPORTED, "gradient norm: too many tensors in one call");
+        a.partials = partials + used;
+        LaunchScope scope(K_GRAD_NORM, bytes, stream);
+        norm_partial_kernel<kCapNorm><<<grid, kThreads, 0, stream>>>(a);
+        MB_CUDA_CHECK(cudaGetLastError());
+        used += grid;
+        return OK;
+      });
+  *n_partials = used;
+  return rc;
+}
+
+template <typename T, int KIND, bool TO_CODES, int CAP>
+int convert_launch(void* const* x, void* const* codes, void* const* scales, const int64_t* numel, int count,
+                   cudaStream_t stream) {
+  ConvertArgs<CAP> a;
+  int n = 0;
+  double elems = 0;
+  a.start[0] = 0;
+  for (int i = 0; i <= count; ++i) {
+    const int64_t per = (int64_t)kBlocksPerChunk * kStateBlock;
+    const int64_t chunks = i < count ? (numel[i] + per - 1) / per : 0;
+    if (i == count || n == CAP || !fits(a.start[n], chunks)) {
+      if (n > 0) {
+        a.count = n;
+        LaunchScope scope(K_STATE_CONVERT, elems * (sizeof(T) + 1.0 + 4.0 / kStateBlock), stream);
+        convert_kernel<T, KIND, TO_CODES, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
+        MB_CUDA_CHECK(cudaGetLastError());
+      }
+      n = 0;
+      elems = 0;
+    }
+    if (chunks == 0) continue;
+    a.x[n] = x[i];
+    a.codes[n] = static_cast<uint8_t*>(codes[i]);
+    a.scales[n] = static_cast<float*>(scales[i]);
+    a.numel[n] = numel[i];
+    a.vec_ok[n] = aligned(x[i], 16) && aligned(codes[i], 8);
+    a.start[n + 1] = a.start[n] + (int)chunks;
+    elems += (double)numel[i];
+    ++n;
+  }
+  return OK;
+}
+
+template <bool TO_CODES>
+int convert(void* const* x, void* const* codes, void* const* scales, const int64_t* numel, int count, int dtype,
+            int kind, cudaStream_t stream) {
+  const bool avg = kind == STATE_EXP_AVG;
+#define MB_CONVERT(T)                                                                                       \
+  return avg ? convert_launch<T, STATE_EXP_AVG, TO_CODES, kCapConvert>(x, codes, scales, numel, count, stream) \
+             : convert_launch<T, STATE_EXP_AVG_SQ, TO_CODES, kCapConvert>(x, codes, scales, numel, count, stream)
+  if (dtype == DT_F32) MB_CONVERT(float);
+  if (dtype == DT_BF16) MB_CONVERT(__nv_bfloat16);
+  MB_CONVERT(__half);
+#undef MB_CONVERT
+}
+
+}  // namespace
+
+int run_adamw(const AdamWCall& c, cudaStream_t stream) {
+  AdamWConsts k;
+  k.b1 = (float)c.beta1;
+  k.w1 = (float)(1.0 - c.beta1);
+  k.b2 = (float)c.beta2;
+  k.w2 = (float)(1.0 - c.beta2);
+  k.eps = (float)c.eps;
+  k.decay = (float)(1.0 - c.lr * c.weight_decay);
+  k.grad_scale = c.grad_scale;
+  k.count = 0;
+  const bool wide = c.grad_dtype == DT_F32;
+  if (c.param_dtype == DT_F32) return adamw_launch<float, float>(c, k, stream);
+  if (c.param_dtype == DT_BF16)
+    return wide ? adamw_launch<__nv_bfloat16, float>(c, k, stream) : adamw_launch<__nv_bfloat16, __nv_bfloat16>(c, k, stream);
+  return wide ? adamw_launch<__half, float>(c, k, stream) : adamw_launch<__half, __half>(c, k, stream);
+}
+
+int grad_norm_partials(int* n) {
+  int sms = 0;
+  const int rc = device_sm_count(&sms);
+  *n = sms * kNormBlocksPerSm * kNormTables;
+  return rc;
+}
+
+int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                  float* out2, double* partials, cudaStream_t stream) {
+  int n = 0;
+  const int rc = norm_partials(tensors, numel, dtypes, count, partials, &n, stream);
+  if (rc != OK) return rc;
+  LaunchScope scope(K_GRAD_NORM, 8.0 * n, stream);
+  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, n, (float)max_norm, out2);
+  MB_CUDA_CHECK(cudaGetLastError());
+  return OK;
+}
+
+int run_clip(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+             float* out2, double* partials, cudaStream_t stream) {
+  int n = 0, launched = 0;
+  int rc = norm_partials(tensors, numel, dtypes, count, partials, &n, stream);
+  if (rc != OK) return rc;
+  rc = for_each_norm_table<kCapNorm>(
+      tensors, numel, dtypes, count, partials, [&](NormArgs<kCapNorm>& a, double bytes) -> int {
+        int grid = 0;
+        const int rc = norm_grid(a.chunks, &grid);
+        if (rc != OK) return rc;
+        ++launched;
+        LaunchScope scope(K_GRAD_NORM, 2.0 * bytes, stream);
+        clip_kernel<kCapNorm><<<grid, kThreads, 0, stream>>>(a, n, (float)max_norm, out2);
+        MB_CUDA_CHECK(cudaGetLastError());
+        return OK;
+      });
+  if (rc != OK || launched) return rc;
+  LaunchScope scope(K_GRAD_NORM, 0.0, stream);  // nothing but empty tensors: the norm is 0
+  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, 0, (float)max_norm, out2);
+  MB_CUDA_CHECK(cudaGetLastError());
+  return OK;
+}
+
+int run_quantize(void* const* src, void* const* codes, void* const* scales, const int64_t* numel, int count,
+                 int dtype, int kind, cudaStream_t stream) {
+  return convert<true>(src, codes, scales, numel, count, dtype, kind, stream);
+}
+
+int run_dequantize(void* const* codes, void* const* scales, void* const* dst, const int64_t* numel, int count,
+                   int dtype, int kind, cudaStream_t stream) {
+  return convert<false>(dst, codes, scales, numel, count, dtype, kind, stream);
+}
+
+}  // namespace mb

@@ -3,6 +3,7 @@
 // entry point replaces are in include/muon_b200.h.
 #include "../../include/muon_b200.h"
 
+#include "adamw.h"
 #include "common.cuh"
 #include "elementwise.h"
 #include "ns_driver.h"
@@ -542,6 +543,161 @@ int muon_b200_adam(void* const* params, void* const* grads, void* const* exp_avg
     if (rc != OK) return rc;
   }
   return OK;
+}
+
+namespace {
+// Checks that the multi-tensor AdamW, norm and conversion entry points share. A tensor without elements may
+// have null pointers. 2^40 elements keep every chunk count within an int.
+int check_list(const char* what, const int64_t* numel, int count) {
+  if (count < 0) return set_error(ERR_INVALID_ARG, "%s: count is negative", what);
+  if (count > 0 && !numel) return set_error(ERR_INVALID_ARG, "%s: numel is NULL", what);
+  for (int i = 0; i < count; ++i)
+    if (numel[i] < 0 || numel[i] > (int64_t)1 << 40)
+      return set_error(ERR_INVALID_ARG, "%s: tensor %d has %lld elements", what, i, (long long)numel[i]);
+  return OK;
+}
+int check_pointers(const char* what, const char* name, void* const* ptrs, const int64_t* numel, int count,
+                   uintptr_t bytes) {
+  if (count > 0 && !ptrs) return set_error(ERR_INVALID_ARG, "%s: %s is NULL", what, name);
+  for (int i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    if (!ptrs[i]) return set_error(ERR_INVALID_ARG, "%s: tensor %d has a null %s", what, i, name);
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) & (bytes - 1))
+      return set_error(ERR_ALIGNMENT, "%s: %s of tensor %d is not aligned to its elements", what, name, i);
+  }
+  return OK;
+}
+uintptr_t elem_size(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+// Everything about an AdamW call but its moments.
+int check_adamw(const char* what, const AdamWCall& c, bool has_masters) {
+  int rc;
+  if ((rc = check_dtype(c.param_dtype)) != OK || (rc = check_dtype(c.grad_dtype)) != OK) return rc;
+  if (c.grad_dtype != c.param_dtype && c.grad_dtype != DT_F32)
+    return set_error(ERR_INVALID_ARG, "%s: gradients have the parameters' type or float32", what);
+  if (has_masters && c.param_dtype == DT_F32)
+    return set_error(ERR_INVALID_ARG, "%s: a float32 parameter has no master weight", what);
+  if (!(c.beta1 >= 0 && c.beta1 < 1) || !(c.beta2 >= 0 && c.beta2 < 1))
+    return set_error(ERR_INVALID_ARG, "%s: betas must be in [0, 1)", what);
+  if (!(c.eps >= 0)) return set_error(ERR_INVALID_ARG, "%s: eps must not be negative", what);
+  if (reinterpret_cast<uintptr_t>(c.grad_scale) & 3)
+    return set_error(ERR_ALIGNMENT, "%s: grad_scale is not aligned to a float", what);
+  if ((rc = check_list(what, c.numel, c.count)) != OK) return rc;
+  if (c.count > 0 && !c.steps) return set_error(ERR_INVALID_ARG, "%s: steps is NULL", what);
+  for (int i = 0; i < c.count; ++i)
+    if (c.steps[i] < 1) return set_error(ERR_INVALID_ARG, "%s: tensor %d has step %lld, steps count from 1", what, i,
+                                         (long long)c.steps[i]);
+  if ((rc = check_pointers(what, "parameter", c.param, c.numel, c.count, elem_size(c.param_dtype))) != OK ||
+      (rc = check_pointers(what, "gradient", c.grad, c.numel, c.count, elem_size(c.grad_dtype))) != OK)
+    return rc;
+  return has_masters ? check_pointers(what, "master weight", c.master, c.numel, c.count, 4) : OK;
+}
+
+int check_norm(const char* what, void* const* tensors, const int64_t* numel, const int* dtypes, int count,
+               double max_norm, const float* out2, const void* scratch, int64_t scratch_bytes) {
+  int rc = check_list(what, numel, count);
+  if (rc != OK) return rc;
+  if (count > 0 && !dtypes) return set_error(ERR_INVALID_ARG, "%s: dtypes is NULL", what);
+  for (int i = 0; i < count; ++i) {
+    if ((rc = check_dtype(dtypes[i])) != OK) return rc;
+    if (numel[i] && !tensors) return set_error(ERR_INVALID_ARG, "%s: tensors is NULL", what);
+    if (numel[i] && (rc = check_pointers(what, "tensor", tensors + i, numel + i, 1, elem_size(dtypes[i]))) != OK) return rc;
+  }
+  if (!(max_norm >= 0)) return set_error(ERR_INVALID_ARG, "%s: max_norm must not be negative", what);
+  if (!out2 || !scratch) return set_error(ERR_INVALID_ARG, "%s: null output or scratch", what);
+  if ((reinterpret_cast<uintptr_t>(out2) & 3) || (reinterpret_cast<uintptr_t>(scratch) & 255))
+    return set_error(ERR_ALIGNMENT, "%s: scratch must be 256-byte aligned, the output 4-byte aligned", what);
+  const int64_t need = muon_b200_grad_norm_scratch_bytes();
+  if (need < 0) return (int)need;
+  if (scratch_bytes < need)
+    return set_error(ERR_INVALID_ARG, "%s: scratch too small: %lld bytes given, %lld needed", what,
+                     (long long)scratch_bytes, (long long)need);
+  return OK;
+}
+
+int check_state(const char* what, void* const* x, void* const* codes, void* const* scales, const int64_t* numel,
+                int count, int dtype, int kind) {
+  int rc = check_dtype(dtype);
+  if (rc != OK) return rc;
+  if (kind != MUON_B200_EXP_AVG && kind != MUON_B200_EXP_AVG_SQ)
+    return set_error(ERR_INVALID_ARG, "%s: unknown kind of state %d", what, kind);
+  if ((rc = check_list(what, numel, count)) != OK ||
+      (rc = check_pointers(what, "tensor", x, numel, count, elem_size(dtype))) != OK ||
+      (rc = check_pointers(what, "code tensor", codes, numel, count, 1)) != OK)
+    return rc;
+  return check_pointers(what, "scale tensor", scales, numel, count, 4);
+}
+}  // namespace
+
+int muon_b200_adamw(void* const* params, void* const* masters, void* const* grads, void* const* exp_avg,
+                    void* const* exp_avg_sq, const int64_t* numel, const int64_t* steps, int count,
+                    int param_dtype, int grad_dtype, double lr, double weight_decay, double beta1,
+                    double beta2, double eps, const float* grad_scale, muon_b200_stream_t stream) {
+  const AdamWCall c{params, masters, grads, exp_avg, nullptr, exp_avg_sq, nullptr, numel, steps, count, param_dtype,
+                    grad_dtype, lr, weight_decay, beta1, beta2, eps, grad_scale, 0};
+  int rc = check_adamw("adamw", c, masters != nullptr);
+  if (rc != OK || (rc = check_pointers("adamw", "exp_avg", exp_avg, numel, count, 4)) != OK ||
+      (rc = check_pointers("adamw", "exp_avg_sq", exp_avg_sq, numel, count, 4)) != OK)
+    return rc;
+  int sms = 0;
+  if (count == 0 || (rc = device_sm_count(&sms)) != OK) return rc;
+  return run_adamw(c, as_stream(stream));
+}
+
+int muon_b200_adamw8(void* const* params, void* const* masters, void* const* grads,
+                     void* const* exp_avg_codes, void* const* exp_avg_scales,
+                     void* const* exp_avg_sq_codes, void* const* exp_avg_sq_scales, const int64_t* numel,
+                     const int64_t* steps, int count, int param_dtype, int grad_dtype, double lr,
+                     double weight_decay, double beta1, double beta2, double eps, uint32_t seed,
+                     const float* grad_scale, muon_b200_stream_t stream) {
+  const AdamWCall c{params, masters, grads, exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales, numel,
+                    steps, count, param_dtype, grad_dtype, lr, weight_decay, beta1, beta2, eps, grad_scale, seed};
+  int rc = check_adamw("adamw8", c, masters != nullptr);
+  if (rc != OK) return rc;
+  if (!(eps >= 1e-16))
+    return set_error(ERR_INVALID_ARG, "adamw8: eps must be at least 1e-16 (8-bit moments below 2^-120 count as 0)");
+  if ((rc = check_pointers("adamw8", "exp_avg code tensor", exp_avg_codes, numel, count, 1)) != OK ||
+      (rc = check_pointers("adamw8", "exp_avg scale tensor", exp_avg_scales, numel, count, 4)) != OK ||
+      (rc = check_pointers("adamw8", "exp_avg_sq code tensor", exp_avg_sq_codes, numel, count, 1)) != OK ||
+      (rc = check_pointers("adamw8", "exp_avg_sq scale tensor", exp_avg_sq_scales, numel, count, 4)) != OK)
+    return rc;
+  int sms = 0;
+  if (count == 0 || (rc = device_sm_count(&sms)) != OK) return rc;
+  return run_adamw(c, as_stream(stream));
+}
+
+int64_t muon_b200_grad_norm_scratch_bytes(void) {
+  int n = 0;
+  const int rc = grad_norm_partials(&n);
+  return rc == OK ? (int64_t)n * 8 : rc;
+}
+
+int muon_b200_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                        float* out2, void* scratch, int64_t scratch_bytes, muon_b200_stream_t stream) {
+  const int rc = check_norm("grad_norm", tensors, numel, dtypes, count, max_norm, out2, scratch, scratch_bytes);
+  if (rc != OK) return rc;
+  return run_grad_norm(tensors, numel, dtypes, count, max_norm, out2, static_cast<double*>(scratch), as_stream(stream));
+}
+
+int muon_b200_clip_grads(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                         float* out2, void* scratch, int64_t scratch_bytes, muon_b200_stream_t stream) {
+  const int rc = check_norm("clip_grads", tensors, numel, dtypes, count, max_norm, out2, scratch, scratch_bytes);
+  if (rc != OK) return rc;
+  return run_clip(tensors, numel, dtypes, count, max_norm, out2, static_cast<double*>(scratch), as_stream(stream));
+}
+
+int muon_b200_quantize_state(void* const* src, void* const* codes, void* const* scales, const int64_t* numel,
+                             int count, int dtype, int kind, muon_b200_stream_t stream) {
+  int rc = check_state("quantize_state", src, codes, scales, numel, count, dtype, kind), sms = 0;
+  if (rc != OK || count == 0 || (rc = device_sm_count(&sms)) != OK) return rc;
+  return run_quantize(src, codes, scales, numel, count, dtype, kind, as_stream(stream));
+}
+
+int muon_b200_dequantize_state(void* const* codes, void* const* scales, void* const* dst, const int64_t* numel,
+                               int count, int dtype, int kind, muon_b200_stream_t stream) {
+  int rc = check_state("dequantize_state", dst, codes, scales, numel, count, dtype, kind), sms = 0;
+  if (rc != OK || count == 0 || (rc = device_sm_count(&sms)) != OK) return rc;
+  return run_dequantize(codes, scales, dst, numel, count, dtype, kind, as_stream(stream));
 }
 
 }  // extern "C"

@@ -15,7 +15,10 @@ enum KernelKind : int {
   K_AOL_RESCALE = 5,
   K_FRO_NORMALIZE = 6,
   K_ADAM = 7,
-  K_KIND_COUNT = 8,
+  K_ADAMW = 8,          // AdamW with 32-bit or 8-bit moments
+  K_GRAD_NORM = 9,      // global norm, clipping
+  K_STATE_CONVERT = 10, // moments 32-bit <-> 8-bit
+  K_KIND_COUNT = 11,
 };
 
 // Counts the launch; when timing is enabled also brackets it with two events recorded on

@@ -13,13 +13,15 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from typing import Sequence
 
 import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import BF16, F16, F32, F64, NS_AOL4, NS_AOL4_FP8, NS_CLASSIC5, NS_HAVE_SUMSQ, check, i64_array, lib, ptr_array
+from ._lib import (BF16, EXP_AVG, EXP_AVG_SQ, F16, F32, F64, NS_AOL4, NS_AOL4_FP8, NS_CLASSIC5, NS_HAVE_SUMSQ,
+                   STATE_BLOCK, address, check, i64_array, lib, ptr_array)
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 # element types the cast at the entry of Newton-Schulz accepts (muon.py:760 takes any float dtype)
@@ -202,6 +204,83 @@ def ramped_sizes(sizes: list[int], growth: float = 0.25) -> list[int]:
         cuts = [round(i * left / groups) for i in range(groups + 1)]
         out.extend(e - s for s, e in zip(cuts[:-1], cuts[1:]))
     return out
+
+
+# ---- tables of many tensors (AdamW, gradient norm, state conversion) --------------------
+# One C-level call per tensor and property: with hundreds of tensors the checks of a call would
+# otherwise take longer than its kernel.
+_dtype_of = Tensor.dtype.__get__
+_STATE_KINDS = {"exp_avg": EXP_AVG, "exp_avg_sq": EXP_AVG_SQ}
+
+
+def _dense(t: Tensor) -> bool:
+    """Every element of `t` at a place of its own, without gaps (any order of dimensions)."""
+    at = 1
+    for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz != 1):
+        if stride != at and t.numel() > 0:
+            return False
+        at *= size
+    return True
+
+
+def state_blocks(numel) -> array:
+    """Scales that 8-bit state of tensors of these sizes has."""
+    return array("q", [-(-n // STATE_BLOCK) for n in numel])
+
+
+class _Tables:
+    """Pointer tables of one call: lists of tensors that are read or written together, element by
+    element in the order of memory. All on one device; written tensors all different."""
+
+    def __init__(self, what: str, first: Sequence[Tensor]):
+        self.what, self.n = what, len(first)
+        self.device_index = first[0].get_device()
+        _require_cuda(first[0], f"every tensor of {what}")
+        self.device = first[0].device
+        self.numel = array("q", map(Tensor.numel, first))
+        self._first, self._strided, self._written, self._n_written = first, False, set(), 0
+
+    def add(self, name: str, tensors: Sequence[Tensor], dtypes=None, numel=None, written: bool = False) -> array:
+        """Table of addresses. `dtypes`: the element types allowed; `numel`: sizes (default: those of
+        the first list, whose memory order the tensors must then share)."""
+        if len(tensors) != self.n:
+            raise ValueError(f"{self.what}: {len(tensors)} {name} tensors for {self.n} tensors")
+        if set(map(Tensor.get_device, tensors)) != {self.device_index}:
+            for t in tensors:
+                _require_cuda(t, f"every {name} tensor of {self.what}")
+            raise ValueError(f"{self.what}: {name} tensors must all be on {self.device}")
+        found = set(map(_dtype_of, tensors))
+        if dtypes is not None and not found <= dtypes:
+            raise ValueError(f"{self.what}: {name} tensors must be {' or '.join(sorted(map(str, dtypes)))}, "
+                             f"got {', '.join(sorted(map(str, found - dtypes)))}")
+        if (self.numel if numel is None else numel) != array("q", map(Tensor.numel, tensors)):
+            raise ValueError(f"{self.what}: a {name} tensor has another number of elements than it must have")
+        if self._strided or not all(map(Tensor.is_contiguous, tensors)):
+            self._check_strides(name, tensors, numel is not None)
+        table = array("Q", map(Tensor.data_ptr, tensors))
+        if written:
+            self._written.update(table)
+            self._n_written += self.n
+            if len(self._written) != self._n_written:
+                self._check_overlap(name)
+        return table
+
+    def _check_strides(self, name, tensors, own_layout: bool) -> None:
+        if tensors is self._first:
+            self._strided = True
+        for t, ref in zip(tensors, self._first):
+            if t.is_contiguous() and (own_layout or ref.is_contiguous()):
+                continue
+            if own_layout or t.stride() != ref.stride() or not _dense(t):
+                raise ValueError(f"{self.what}: {name} tensors must be contiguous, or dense with the strides of the "
+                                 f"tensor they belong to; got shape {tuple(t.shape)}, strides {t.stride()}")
+
+    def _check_overlap(self, name) -> None:
+        """Two written tensors at one address: only tensors without elements may be."""
+        self._written.discard(0)
+        empty = sum(1 for n in self.numel if n == 0)
+        if empty == 0 or len(self._written) < self._n_written - empty * (self._n_written // self.n):
+            raise ValueError(f"{self.what}: a tensor that is written ({name}) appears twice in the call")
 
 
 class CudaBackend:
@@ -533,6 +612,110 @@ class CudaBackend:
                 ptr_array([m.data_ptr() for m in exp_avgs]), ptr_array([v.data_ptr() for v in exp_avg_sqs]),
                 i64_array([p.numel() for p in params]), i64_array(list(steps)), len(params), code,
                 lr, weight_decay, betas[0], betas[1], eps, _stream_ptr(dev)))
+            self.launch_groups += 1
+
+    # -- AdamW, moments in 32 or 8 bits; gradient norm (adamw.py) --------------------------
+    @staticmethod
+    def _adamw_tables(what, params, grads, masters, steps, grad_scale):
+        """(tables, parameter / gradient / master addresses, steps, dtype codes, factor) of a call."""
+        tab = _Tables(what, params)
+        p = tab.add("parameter", params, written=True)
+        kinds = set(map(_dtype_of, params))
+        code = dtype_code(params[0])
+        if len(kinds) != 1:
+            raise ValueError(f"{what} needs parameters of one dtype, got {', '.join(sorted(map(str, kinds)))}")
+        g = tab.add("gradient", grads, kinds | {torch.float32})
+        if len(set(map(_dtype_of, grads))) != 1:
+            raise ValueError(f"{what} needs gradients of one dtype")
+        w = None if masters is None else tab.add("master", masters, {torch.float32}, written=True)
+        if masters is not None and code == F32:
+            raise ValueError(f"{what}: float32 parameters have no master weights")
+        steps = array("q", [steps]) * tab.n if isinstance(steps, int) else array("q", steps)
+        if len(steps) != tab.n:
+            raise ValueError(f"{what}: {len(steps)} steps for {tab.n} tensors")
+        if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1
+                                       or grad_scale.get_device() != tab.device_index):
+            raise ValueError(f"{what}: grad_scale must be one float32 value on {tab.device}")
+        return tab, p, g, w, steps, code, dtype_code(grads[0]), None if grad_scale is None else grad_scale.data_ptr()
+
+    def adamw_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
+                   exp_avg_sqs: Sequence[Tensor], steps, lr: float, weight_decay: float, betas: tuple[float, float],
+                   eps: float, masters=None, grad_scale: Tensor | None = None) -> None:
+        """AdamW with float32 moments on tensors of any sizes; one parameter and one gradient dtype."""
+        if not params:
+            return
+        tab, p, g, w, steps, code, g_code, factor = self._adamw_tables("adamw_step", params, grads, masters, steps,
+                                                                       grad_scale)
+        m = tab.add("exp_avg", exp_avgs, {torch.float32}, written=True)
+        v = tab.add("exp_avg_sq", exp_avg_sqs, {torch.float32}, written=True)
+        with torch.cuda.device(tab.device_index):
+            _wait_grads(torch.cuda.current_stream(tab.device), grads)
+            check(lib.muon_b200_adamw(
+                address(p), None if w is None else address(w), address(g), address(m), address(v), address(tab.numel),
+                address(steps), tab.n, code, g_code, lr, weight_decay, betas[0], betas[1], eps, factor,
+                _stream_ptr(tab.device)))
+            self.launch_groups += 1
+
+    def adamw8_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg_codes: Sequence[Tensor],
+                    exp_avg_scales: Sequence[Tensor], exp_avg_sq_codes: Sequence[Tensor],
+                    exp_avg_sq_scales: Sequence[Tensor], steps, lr: float, weight_decay: float,
+                    betas: tuple[float, float], eps: float, masters=None, grad_scale: Tensor | None = None,
+                    seed: int = 0) -> None:
+        """AdamW with moments in 8 bits (codes of the parameter's size, one float32 scale per 256)."""
+        if not params:
+            return
+        tab, p, g, w, steps, code, g_code, factor = self._adamw_tables("adamw8_step", params, grads, masters, steps,
+                                                                       grad_scale)
+        blocks = state_blocks(tab.numel)
+        m = tab.add("exp_avg code", exp_avg_codes, {torch.uint8}, written=True)
+        ms = tab.add("exp_avg scale", exp_avg_scales, {torch.float32}, blocks, written=True)
+        v = tab.add("exp_avg_sq code", exp_avg_sq_codes, {torch.uint8}, written=True)
+        vs = tab.add("exp_avg_sq scale", exp_avg_sq_scales, {torch.float32}, blocks, written=True)
+        with torch.cuda.device(tab.device_index):
+            _wait_grads(torch.cuda.current_stream(tab.device), grads)
+            check(lib.muon_b200_adamw8(
+                address(p), None if w is None else address(w), address(g), address(m), address(ms), address(v),
+                address(vs), address(tab.numel), address(steps), tab.n, code, g_code, lr, weight_decay, betas[0],
+                betas[1], eps, seed & 0xFFFFFFFF, factor, _stream_ptr(tab.device)))
+            self.launch_groups += 1
+
+    def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> Tensor:
+        """{norm, factor} of all `tensors` together, on their device; with `clip` the tensors are
+        multiplied by the factor."""
+        what = "clip_grad_norm_" if clip else "grad_norm"
+        tab = _Tables(what, tensors)
+        x = tab.add("gradient", tensors, set(_DTYPE_CODE), written=clip)
+        codes = array("i", [_DTYPE_CODE[d] for d in map(_dtype_of, tensors)])
+        with torch.cuda.device(tab.device_index):
+            _wait_grads(torch.cuda.current_stream(tab.device), tensors)
+            out = torch.empty(2, dtype=torch.float32, device=tab.device)
+            need = lib.muon_b200_grad_norm_scratch_bytes()
+            # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
+            # one stream may be replayed at the same time on two.
+            scratch = (torch.empty(need + 256, dtype=torch.uint8, device=tab.device)
+                       if torch.cuda.is_current_stream_capturing() else self.workspace(tab.device, need, slot=5))
+            call = lib.muon_b200_clip_grads if clip else lib.muon_b200_grad_norm
+            check(call(address(x), address(tab.numel), address(codes), tab.n, max_norm, out.data_ptr(),
+                       self._aligned_ptr(scratch), need, _stream_ptr(tab.device)))
+            self.launch_groups += 1
+        return out
+
+    def convert_state(self, what: str, values: Sequence[Tensor], codes: Sequence[Tensor], scales: Sequence[Tensor],
+                      kind: str, to_codes: bool) -> None:
+        """Values <-> 8-bit codes and scales, one dtype of values per call."""
+        if not codes:
+            return
+        tab = _Tables(what, codes)
+        c = tab.add("code", codes, {torch.uint8}, written=to_codes)
+        s = tab.add("scale", scales, {torch.float32}, state_blocks(tab.numel), written=to_codes)
+        x = tab.add("value", values, set(_DTYPE_CODE), written=not to_codes)
+        if len(set(map(_dtype_of, values))) != 1:
+            raise ValueError(f"{what} needs values of one dtype")
+        tables = (x, c, s) if to_codes else (c, s, x)
+        call = lib.muon_b200_quantize_state if to_codes else lib.muon_b200_dequantize_state
+        with torch.cuda.device(tab.device_index):
+            check(call(*map(address, tables), address(tab.numel), tab.n, dtype_code(values[0]), _STATE_KINDS[kind],
+                       _stream_ptr(tab.device)))
             self.launch_groups += 1
 
     # -- functional pieces -------------------------------------------------------------
