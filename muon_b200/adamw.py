@@ -14,7 +14,8 @@ from typing import Sequence
 import torch
 from torch import Tensor
 
-from .engine import _STATE_KINDS, get_backend, state_blocks
+from ._lib import STATE_BLOCK
+from .engine import _STATE_KINDS, get_backend
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
@@ -99,8 +100,7 @@ def quantize_state(tensors: Sequence[Tensor], kind: str, *, codes: Sequence[Tens
     if codes is None:
         codes = [torch.empty_like(t, dtype=torch.uint8) for t in tensors]
     if scales is None:
-        scales = [torch.empty(n, dtype=torch.float32, device=t.device)
-                  for t, n in zip(tensors, state_blocks(t.numel() for t in tensors))]
+        scales = [torch.empty(-(-t.numel() // STATE_BLOCK), dtype=torch.float32, device=t.device) for t in tensors]
     get_backend().convert_state("quantize_state", tensors, codes, scales, kind, True)
     return codes, scales
 

@@ -1,24 +1,31 @@
-"""Builds ``libmuon_b200.so`` (the C-ABI CUDA library) in-tree with nvcc for sm_100a.
+"""Builds ``libmuon_b200.so`` (the C-ABI CUDA library) and ``_tables.so`` (the Python extension that
+lays out pointer tables) in-tree, with nvcc for sm_100a and the host compiler.
 
 Usage: ``python muon_b200/build.py [--force] [-v]``. Run it as a script: importing the
 package needs the library to exist already. nvcc cross-compiles, so no GPU is needed.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmuon_b200.so")
+TABLES_PATH = os.path.join(PKG_DIR, "_tables.so")
 SOURCES = ("api.cu", "ns_driver.cu", "ns_gemm.cu", "elementwise.cu", "adamw.cu", "profiling.cu", "peer.cu", "no_alloc.cu")
 HEADERS = ("common.cuh", "ns_driver.h", "ns_gemm.h", "elementwise.h", "adamw.h", "profiling.h", os.path.join("..", "..", "include", "muon_b200.h"))
+TABLES_SOURCE = "tables.cpp"
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 )
 
 
@@ -29,28 +36,60 @@ def _nvcc() -> str:
     return exe
 
 
-def is_stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _older(target: str, names) -> bool:
+    if not os.path.exists(target):
         return True
-    built = os.path.getmtime(LIB_PATH)
-    deps = [os.path.join(CSRC, s) for s in SOURCES + HEADERS]
+    built = os.path.getmtime(target)
+    deps = [os.path.join(CSRC, s) for s in names]
     return any(os.path.getmtime(d) > built for d in deps if os.path.exists(d))
 
 
-def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if it is missing or older than its sources. Returns its path."""
-    if not force and not is_stale():
-        return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", LIB_PATH, *[os.path.join(CSRC, s) for s in SOURCES]]
+def is_stale() -> bool:
+    return _older(LIB_PATH, SOURCES + HEADERS) or _older(TABLES_PATH, (TABLES_SOURCE,))
+
+
+def _run(cmd, verbose: bool = False) -> None:
     if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
         print(" ".join(cmd), file=sys.stderr)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     if verbose:
         print(proc.stderr, file=sys.stderr)
+
+
+def _build_tables(verbose: bool) -> None:
+    spec = importlib.util.find_spec("torch")  # the path alone: torch need not be imported to build
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("PyTorch not found: cannot build _tables.so")
+    torch_dir = list(spec.submodule_search_locations)[0]
+    include = os.path.join(torch_dir, "include")
+    compiler = shutil.which("g++") or shutil.which("c++")
+    if compiler is None:
+        raise RuntimeError("no C++ compiler found: cannot build _tables.so")
+    _run([compiler, "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + include,
+          "-I" + os.path.join(include, "torch", "csrc", "api", "include"),
+          "-I" + sysconfig.get_paths()["include"], "-o", TABLES_PATH, os.path.join(CSRC, TABLES_SOURCE),
+          "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], verbose)
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
+    """Compile what is missing or older than its sources, files side by side. Returns the library's path."""
+    jobs = []
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor() as pool:
+        if force or _older(TABLES_PATH, (TABLES_SOURCE,)):
+            jobs.append(pool.submit(_build_tables, verbose))
+        objects = []
+        if force or _older(LIB_PATH, SOURCES + HEADERS):
+            for name in SOURCES:
+                objects.append(os.path.join(tmp, name + ".o"))
+                extra = ["-Xptxas", "-v"] if verbose else []
+                jobs.append(pool.submit(_run, [_nvcc(), *extra, *NVCC_FLAGS, "-c", "-o", objects[-1],
+                                               os.path.join(CSRC, name)], verbose))
+        for job in jobs:
+            job.result()
+        if objects:
+            _run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects], verbose)
     return LIB_PATH
 
 

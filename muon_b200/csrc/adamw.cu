@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <cmath>
+#include <type_traits>
 
 namespace mb {
 
@@ -97,7 +98,29 @@ struct Raw {  // the words of N elements, as loaded
       w[k] = make_uint4(u[0], u[1], u[2], u[3]);
     }
   }
+  __device__ __forceinline__ void unpack(float2 (&v)[N / 2]) const {
+    float x[N];
+    unpack(x);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) v[j] = make_float2(x[2 * j], x[2 * j + 1]);
+  }
+  __device__ __forceinline__ void pack(const float2 (&v)[N / 2]) {
+    float x[N];
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      x[2 * j] = v[j].x;
+      x[2 * j + 1] = v[j].y;
+    }
+    pack(x);
+  }
 };
+
+// Two float32 operations in one instruction, one rounding each.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+// a + b where a is a product: as a multiply-add by a 1 that the compiler does not know (the assembler
+// fuses a paired product and a paired sum into one operation with one rounding, unlike single ones).
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) { return __ffma2_rn(a, both(one), b); }
 
 __device__ __forceinline__ float sqrt_approx(float x) {  // relative error at most 2^-23
   float r;
@@ -120,6 +143,7 @@ __device__ __forceinline__ int find_tensor(const S& start, int count, int chunk)
 struct AdamWConsts {
   float b1, w1, b2, w2;  // float(beta), float(1 - beta)
   float eps, decay;      // decay = float(1 - lr * weight_decay)
+  float one;             // 1 (see add2)
   const float* grad_scale;
   int count;
 };
@@ -261,61 +285,93 @@ __device__ __forceinline__ void block_scale(float amax, float& scale, float& inv
   inv = tiny ? 0.f : __fdiv_rn(top, amax);
 }
 
-// Largest |x| of a warp's eight elements a lane, by the bits: a NaN is above everything.
-__device__ __forceinline__ float warp_amax(const float (&x)[8]) {
-  uint32_t b = 0;
+// Largest |x| over the warp of the largest of each lane, by the bits: a NaN is above everything.
+__device__ __forceinline__ float warp_max(uint32_t bits) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
+}
+template <int KIND>
+__device__ __forceinline__ uint32_t amax_bits(const float2 (&x)[4]) {
+  uint32_t b[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) b = max(b, __float_as_uint(x[j]) & 0x7fffffffu);
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, b));
+  for (int j = 0; j < 4; ++j) {  // (a second moment has no sign, unless it is -0 or was given one)
+    b[2 * j] = __float_as_uint(x[j].x) & 0x7fffffffu;
+    b[2 * j + 1] = __float_as_uint(x[j].y) & 0x7fffffffu;
+  }
+  return __vimax3_u32(__vimax3_u32(b[0], b[1], b[2]), __vimax3_u32(b[3], b[4], b[5]), max(b[6], b[7]));
 }
 
-__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
-  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-}
+__device__ __forceinline__ uint32_t e4m3_pair(float2 x) { return __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ float2 e4m3_values(uint32_t pair) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-__device__ __forceinline__ float sq_value(uint32_t code) { return __uint_as_float((code + 768u) << 20); }
-__device__ __forceinline__ uint32_t sq_code(float x, uint32_t r) {
-  const int c = ((int)(__float_as_uint(x) + r) >> 20) - 768;
-  return (uint32_t)min(max(c, 0), 255);
+// (code + 768) << 20 of byte j of a word: the offset's bits lie above the code's.
+template <int J>
+__device__ __forceinline__ float sq_value(uint32_t word) {
+  const uint32_t c = J < 3 ? word << (J < 3 ? 20 - 8 * J : 0) : word >> 4;
+  return __uint_as_float((c & 0x0ff00000u) | 0x30000000u);
+}
+__device__ __forceinline__ int sq_cut(float x, uint32_t r) { return (int)(__float_as_uint(x) + r - 0x30000000u) >> 20; }
+// Two integers clamped to 0..255 as bytes 0 and 1, bytes 2 and 3 from the low half of `high`.
+__device__ __forceinline__ uint32_t pack_bytes(int b1, int b0, uint32_t high) {
+  uint32_t d;
+  asm("cvt.pack.sat.u8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(b1), "r"(b0), "r"(high));
+  return d;
 }
 
 // Eight codes of a moment <-> floats.
 template <int KIND>
-__device__ __forceinline__ void decode8(uint2 w, float scale, float (&x)[8]) {
+__device__ __forceinline__ void decode8(uint2 w, float scale, float2 (&x)[4]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint32_t u = h ? w.y : w.x;
     if constexpr (KIND == STATE_EXP_AVG) {
-      const float2 lo = e4m3_values(u & 0xffffu), hi = e4m3_values(u >> 16);
-      x[4 * h] = lo.x; x[4 * h + 1] = lo.y; x[4 * h + 2] = hi.x; x[4 * h + 3] = hi.y;
+      x[2 * h] = e4m3_values(u & 0xffffu);
+      x[2 * h + 1] = e4m3_values(u >> 16);
     } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * h + j] = sq_value((u >> (8 * j)) & 0xffu);
+      x[2 * h] = make_float2(sq_value<0>(u), sq_value<1>(u));
+      x[2 * h + 1] = make_float2(sq_value<2>(u), sq_value<3>(u));
     }
   }
+  const float2 s = make_float2(scale, scale);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], scale);
+  for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], s);
 }
 template <int KIND>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv, const uint32_t (&r)[8]) {
-  uint32_t u[2];
+__device__ __forceinline__ uint2 encode8(const float2 (&x)[4], float inv, const uint32_t (&r)[8]) {
+  const float2 f = make_float2(inv, inv);
+  float2 y[4];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float y[4];
+  for (int j = 0; j < 4; ++j) y[j] = mul2(x[j], f);
+  if constexpr (KIND == STATE_EXP_AVG) {
+    return make_uint2(e4m3_pair(y[0]) | e4m3_pair(y[1]) << 16, e4m3_pair(y[2]) | e4m3_pair(y[3]) << 16);
+  } else {
+    uint32_t u[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(x[4 * h + j], inv);
-    if constexpr (KIND == STATE_EXP_AVG) {
-      u[h] = e4m3_pair(y[0], y[1]) | e4m3_pair(y[2], y[3]) << 16;
-      if (inv == 0.f) u[h] = y[0] == y[0] ? 0u : u[h];
-    } else {
-      u[h] = sq_code(y[0], r[4 * h]) | sq_code(y[1], r[4 * h + 1]) << 8 | sq_code(y[2], r[4 * h + 2]) << 16 |
-             sq_code(y[3], r[4 * h + 3]) << 24;
-    }
+    for (int h = 0; h < 2; ++h)
+      u[h] = pack_bytes(sq_cut(y[2 * h].y, r[4 * h + 1]), sq_cut(y[2 * h].x, r[4 * h]),
+                        pack_bytes(sq_cut(y[2 * h + 1].y, r[4 * h + 3]), sq_cut(y[2 * h + 1].x, r[4 * h + 2]), 0u));
+    return make_uint2(u[0], u[1]);
   }
-  return make_uint2(u[0], u[1]);
+}
+// One code.
+template <int KIND>
+__device__ __forceinline__ float decode1(uint32_t c, float scale) {
+  return __fmul_rn(KIND == STATE_EXP_AVG ? e4m3_values(c).x : sq_value<0>(c), scale);
+}
+__device__ __forceinline__ uint8_t byte_of(uint2 w, int j) { return (uint8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))); }
+
+// Scales of both moments of a block: the two halves of the warp compute one each (a division takes
+// longer than what it is for). Lane 0 and lane 16 return theirs; the factors go to every lane.
+__device__ __forceinline__ float both_scales(float m_amax, float v_amax, int lane, float& m_inv, float& v_inv) {
+  const bool sq = lane >= 16;
+  const float amax = sq ? v_amax : m_amax, top = sq ? kSqMax : kE4m3Max;
+  const bool tiny = amax < (sq ? kTinySq : kTinyAvg);
+  const float scale = tiny ? 0.f : __fmul_rn(amax, sq ? 1.f / kSqMax : 1.f / kE4m3Max);
+  const float inv = tiny ? 0.f : __fdiv_rn(top, amax);
+  m_inv = __shfl_sync(0xffffffffu, inv, 0);
+  v_inv = __shfl_sync(0xffffffffu, inv, 16);
+  return scale;
 }
 
 // 32 random bits for the four elements 4 * word .. 4 * word + 3; element j takes the low 20 bits of
@@ -347,110 +403,161 @@ struct AdamW8Args {
   unsigned char vec_ok[CAP];
 };
 
+constexpr int kBlocksPerSm8 = 4;
 constexpr int kBlocksPerWarp = 4;
 constexpr int kBlocksPerChunk = kWarps * kBlocksPerWarp;
 
+// What a warp needs of a tensor.
+template <typename P, typename G>
+struct Tensor8 {
+  P* p;
+  float* w;
+  const G* g;
+  uint8_t *m, *v;
+  float *ms, *vs;
+  long long numel;
+  float step, rs;
+  uint32_t key;
+};
+
+// New moments and parameters of a lane's eight elements. The moments as the format prescribes, one
+// rounding per operation, two elements per instruction; the update with the hardware's reciprocal
+// (eps is at least 1e-16, so the denominator is a normal number and a second moment too small for
+// one does not matter).
+template <typename T>
+__device__ __forceinline__ void step8(const AdamWConsts& c, const T& t, float f, float2 (&p)[4], float2 (&g)[4],
+                                      float2 (&m)[4], float2 (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    g[j] = mul2(g[j], both(f));
+    m[j] = add2(mul2(m[j], both(c.b1)), mul2(g[j], both(c.w1)), c.one);
+    v[j] = add2(mul2(v[j], both(c.b2)), mul2(mul2(g[j], g[j]), both(c.w2)), c.one);
+    float2 root, inverse;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.x) : "f"(v[j].x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.y) : "f"(v[j].y));
+    const float2 den = __ffma2_rn(root, both(t.rs), both(c.eps));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse.x) : "f"(den.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse.y) : "f"(den.y));
+    p[j] = __ffma2_rn(both(-t.step), mul2(m[j], inverse), mul2(p[j], both(c.decay)));
+  }
+}
+
+// A block that is cut short by the tensor's end, or that does not start on a 16-byte boundary: a lane
+// takes every 32nd element.
+template <typename P, typename G, bool MASTER>
+__device__ __forceinline__ void ragged_block8(const AdamWConsts& c, const Tensor8<P, G>& t, float f, long long b) {
+  const int lane = threadIdx.x & 31;
+  const long long base = b * kStateBlock + lane;
+  const int n = (int)min((long long)kStateBlock, t.numel - b * kStateBlock) - lane;  // this lane's: j with 32 j < n
+  const float ms = t.ms[b], vs = t.vs[b];
+  float2 pj[4], gj[4], mj[4], vj[4];
+  uint32_t r[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool in = 32 * j < n;
+    const long long i = base + 32 * j;
+    float& pe = j & 1 ? pj[j / 2].y : pj[j / 2].x;
+    float& ge = j & 1 ? gj[j / 2].y : gj[j / 2].x;
+    float& me = j & 1 ? mj[j / 2].y : mj[j / 2].x;
+    float& ve = j & 1 ? vj[j / 2].y : vj[j / 2].x;
+    pe = in ? (MASTER ? t.w[i] : to_float<P>(t.p[i])) : 0.f;
+    ge = in ? to_float<G>(t.g[i]) : 0.f;
+    me = in ? decode1<STATE_EXP_AVG>(t.m[i], ms) : 0.f;
+    ve = in ? decode1<STATE_EXP_AVG_SQ>(t.v[i], vs) : 0.f;
+    r[j] = random_bits(random_word((uint32_t)(i >> 2), t.key), (int)(i & 3));
+  }
+  step8(c, t, f, pj, gj, mj, vj);
+  float m_inv, v_inv;
+  const float scale = both_scales(warp_max(amax_bits<STATE_EXP_AVG>(mj)), warp_max(amax_bits<STATE_EXP_AVG_SQ>(vj)),
+                                  lane, m_inv, v_inv);
+  if (lane == 0) t.ms[b] = scale;
+  if (lane == 16) t.vs[b] = scale;
+  const uint2 cm = encode8<STATE_EXP_AVG>(mj, m_inv, r);
+  const uint2 cv = encode8<STATE_EXP_AVG_SQ>(vj, v_inv, r);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const long long i = base + 32 * j;
+    if (32 * j < n) {
+      const float pe = j & 1 ? pj[j / 2].y : pj[j / 2].x;
+      t.m[i] = byte_of(cm, j);
+      t.v[i] = byte_of(cv, j);
+      if (MASTER) t.w[i] = pe;
+      t.p[i] = from_float<P>(pe);
+    }
+  }
+}
+
+// The words of a whole block, eight elements a lane.
+template <typename P, typename G, bool MASTER>
+struct Loaded8 {
+  using W = typename std::conditional<MASTER, float, P>::type;
+  Raw<W, 8> p;
+  Raw<G, 8> g;
+  uint2 m, v;
+  float ms, vs;
+  __device__ __forceinline__ void load(const Tensor8<P, G>& t, long long b, int lane) {
+    const long long at = b * kStateBlock + lane * 8;
+    g.load(t.g + at);
+    if constexpr (MASTER) p.load(t.w + at);
+    else p.load(t.p + at);
+    m = __ldcs(reinterpret_cast<const uint2*>(t.m + at));
+    v = __ldcs(reinterpret_cast<const uint2*>(t.v + at));
+    ms = t.ms[b];
+    vs = t.vs[b];
+  }
+};
+
 template <typename P, typename G, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm8)
 adamw8_kernel(const __grid_constant__ AdamW8Args<CAP> a) {
   float f;
   if (!read_factor(a.c.grad_scale, f)) return;
-  const int t = find_tensor(a.start, a.c.count, (int)blockIdx.x);
+  const int e = find_tensor(a.start, a.c.count, (int)blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long numel = a.numel[t];
-  const long long blocks = (numel + kStateBlock - 1) / kStateBlock;
-  P* p = static_cast<P*>(a.p[t]);
-  float* w = MASTER ? a.w[t] : nullptr;
-  const G* g = static_cast<const G*>(a.g[t]);
-  uint8_t *m = a.m[t], *v = a.v[t];
-  const float step = a.step[t], rs = a.rs[t];
-  const uint32_t key = a.key[t];
+  const Tensor8<P, G> t = {static_cast<P*>(a.p[e]), a.w[e], static_cast<const G*>(a.g[e]), a.m[e], a.v[e], a.ms[e],
+                           a.vs[e], a.numel[e], a.step[e], a.rs[e], a.key[e]};
   const AdamWConsts c = a.c;
-  const long long first = (long long)((int)blockIdx.x - a.start[t]) * kBlocksPerChunk + warp;
-  for (int k = 0; k < kBlocksPerWarp; ++k) {
-    const long long b = first + (long long)k * kWarps;
-    if (b >= blocks) return;
-    const long long base = b * kStateBlock;
-    const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
-    const float ms = a.ms[t][b], vs = a.vs[t][b];
-    float pj[8], gj[8], mj[8], vj[8];
+  const long long blocks = (t.numel + kStateBlock - 1) / kStateBlock;
+  const long long whole = a.vec_ok[e] ? t.numel / kStateBlock : 0;  // blocks that the vector path takes
+  const long long chunk = (long long)((int)blockIdx.x - a.start[e]) * kBlocksPerChunk;
+  const long long end = min(blocks, chunk + kBlocksPerChunk), whole_end = min(whole, end);
+  long long b = chunk + warp;
+  Loaded8<P, G, MASTER> next;
+  if (b < whole_end) next.load(t, b, lane);
+  for (; b < whole_end; b += kWarps) {
+    const Loaded8<P, G, MASTER> now = next;
+    if (b + kWarps < whole_end) next.load(t, b + kWarps, lane);  // under this block's arithmetic
+    const long long at = b * kStateBlock + lane * 8;
+    float2 pj[4], gj[4], mj[4], vj[4];
+    now.p.unpack(pj);
+    now.g.unpack(gj);
+    decode8<STATE_EXP_AVG>(now.m, now.ms, mj);
+    decode8<STATE_EXP_AVG_SQ>(now.v, now.vs, vj);
+    step8(c, t, f, pj, gj, mj, vj);
+    Raw<P, 8> rp;
+    rp.pack(pj);
+    rp.store(t.p + at);
+    if constexpr (MASTER) {
+      Raw<float, 8> rw;
+      rw.pack(pj);
+      rw.store(t.w + at);
+    }
     uint32_t r[8];
-    const long long at = base + lane * 8;  // this lane's elements: eight in a row, or every 32nd
-    if (vec) {
-      Raw<G, 8> rg;
-      rg.load(g + at);
-      if constexpr (MASTER) {
-        Raw<float, 8> rw;
-        rw.load(w + at);
-        rw.unpack(pj);
-      } else {
-        Raw<P, 8> rp;
-        rp.load(p + at);
-        rp.unpack(pj);
-      }
-      const uint2 cm = __ldcs(reinterpret_cast<const uint2*>(m + at));
-      const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(v + at));
-      rg.unpack(gj);
-      decode8<STATE_EXP_AVG>(cm, ms, mj);
-      decode8<STATE_EXP_AVG_SQ>(cv, vs, vj);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t bits = random_word((uint32_t)(at >> 2) + h, key);
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t bits = random_word((uint32_t)(at >> 2) + h, t.key);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) r[4 * h + j] = random_bits(bits, j);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const long long i = base + lane + 32 * j;
-        const bool in = i < numel;
-        pj[j] = in ? (MASTER ? w[i] : to_float<P>(p[i])) : 0.f;
-        gj[j] = in ? to_float<G>(g[i]) : 0.f;
-        mj[j] = in ? __fmul_rn(e4m3_values(m[i]).x, ms) : 0.f;
-        vj[j] = in ? __fmul_rn(sq_value(v[i]), vs) : 0.f;
-        r[j] = random_bits(random_word((uint32_t)(i >> 2), key), (int)(i & 3));
-      }
+      for (int j = 0; j < 4; ++j) r[4 * h + j] = random_bits(bits, j);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      gj[j] = __fmul_rn(gj[j], f);
-      mj[j] = __fadd_rn(__fmul_rn(mj[j], c.b1), __fmul_rn(gj[j], c.w1));
-      vj[j] = __fadd_rn(__fmul_rn(vj[j], c.b2), __fmul_rn(__fmul_rn(gj[j], gj[j]), c.w2));
-      pj[j] = moved(pj[j], mj[j], vj[j], c.decay, step, rs, c.eps);
-    }
-    float m_scale, m_inv, v_scale, v_inv;
-    block_scale<STATE_EXP_AVG>(warp_amax(mj), m_scale, m_inv);
-    block_scale<STATE_EXP_AVG_SQ>(warp_amax(vj), v_scale, v_inv);
-    if (lane == 0) {
-      a.ms[t][b] = m_scale;
-      a.vs[t][b] = v_scale;
-    }
-    const uint2 cm = encode8<STATE_EXP_AVG>(mj, m_inv, r);
-    const uint2 cv = encode8<STATE_EXP_AVG_SQ>(vj, v_inv, r);
-    if (vec) {
-      __stcs(reinterpret_cast<uint2*>(m + at), cm);
-      __stcs(reinterpret_cast<uint2*>(v + at), cv);
-      if constexpr (MASTER) {
-        Raw<float, 8> rw;
-        rw.pack(pj);
-        rw.store(w + at);
-      }
-      Raw<P, 8> rp;
-      rp.pack(pj);
-      rp.store(p + at);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const long long i = base + lane + 32 * j;
-        if (i < numel) {
-          m[i] = (uint8_t)((j < 4 ? cm.x : cm.y) >> (8 * (j & 3)));
-          v[i] = (uint8_t)((j < 4 ? cv.x : cv.y) >> (8 * (j & 3)));
-          if (MASTER) w[i] = pj[j];
-          p[i] = from_float<P>(pj[j]);
-        }
-      }
-    }
+    float m_inv, v_inv;
+    const float scale = both_scales(warp_max(amax_bits<STATE_EXP_AVG>(mj)), warp_max(amax_bits<STATE_EXP_AVG_SQ>(vj)),
+                                    lane, m_inv, v_inv);
+    if (lane == 0) t.ms[b] = scale;
+    if (lane == 16) t.vs[b] = scale;
+    __stcs(reinterpret_cast<uint2*>(t.m + at), encode8<STATE_EXP_AVG>(mj, m_inv, r));
+    __stcs(reinterpret_cast<uint2*>(t.v + at), encode8<STATE_EXP_AVG_SQ>(vj, v_inv, r));
   }
+  for (; b < end; b += kWarps) ragged_block8<P, G, MASTER>(c, t, f, b);
 }
 
 // ---------------------------------------------------------------------------
@@ -465,6 +572,7 @@ struct ConvertArgs {
   int start[CAP + 1];
   unsigned char vec_ok[CAP];
   int count;
+  uint32_t half;  // half a code (2^19), added before the cut: to nearest
 };
 
 template <typename T, int KIND, bool TO_CODES, int CAP>
@@ -485,7 +593,7 @@ convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
     const long long base = b * kStateBlock;
     const long long at = base + lane * 8;
     const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
-    float xj[8];
+    float2 xj[4];
     if constexpr (TO_CODES) {
       if (vec) {
         Raw<T, 8> rx;
@@ -495,14 +603,14 @@ convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const long long i = base + lane + 32 * j;
-          xj[j] = i < numel ? to_float<T>(x[i]) : 0.f;
+          (j & 1 ? xj[j / 2].y : xj[j / 2].x) = i < numel ? to_float<T>(x[i]) : 0.f;
         }
       }
       float scale, inv;
-      block_scale<KIND>(warp_amax(xj), scale, inv);
+      block_scale<KIND>(warp_max(amax_bits<KIND>(xj)), scale, inv);
       if (lane == 0) scales[b] = scale;
-      const uint32_t half = 1u << 19;  // nearest: half a code is added before the cut
-      const uint32_t r[8] = {half, half, half, half, half, half, half, half};
+      // (an argument, because with the constant in its place the compiler's code saturated every value)
+      const uint32_t r[8] = {a.half, a.half, a.half, a.half, a.half, a.half, a.half, a.half};
       const uint2 c = encode8<KIND>(xj, inv, r);
       if (vec) {
         __stcs(reinterpret_cast<uint2*>(codes + at), c);
@@ -510,7 +618,7 @@ convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const long long i = base + lane + 32 * j;
-          if (i < numel) codes[i] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+          if (i < numel) codes[i] = byte_of(c, j);
         }
       }
     } else {
@@ -524,10 +632,7 @@ convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const long long i = base + lane + 32 * j;
-          if (i < numel) {
-            const uint32_t c = codes[i];
-            x[i] = from_float<T>(__fmul_rn(KIND == STATE_EXP_AVG ? e4m3_values(c).x : sq_value(c), scale));
-          }
+          if (i < numel) x[i] = from_float<T>(decode1<KIND>(codes[i], scale));
         }
       }
     }
@@ -860,6 +965,7 @@ template <typename T, int KIND, bool TO_CODES, int CAP>
 int convert_launch(void* const* x, void* const* codes, void* const* scales, const int64_t* numel, int count,
                    cudaStream_t stream) {
   ConvertArgs<CAP> a;
+  a.half = 1u << 19;
   int n = 0;
   double elems = 0;
   a.start[0] = 0;
@@ -912,6 +1018,7 @@ int run_adamw(const AdamWCall& c, cudaStream_t stream) {
   k.w2 = (float)(1.0 - c.beta2);
   k.eps = (float)c.eps;
   k.decay = (float)(1.0 - c.lr * c.weight_decay);
+  k.one = 1.f;
   k.grad_scale = c.grad_scale;
   k.count = 0;
   const bool wide = c.grad_dtype == DT_F32;

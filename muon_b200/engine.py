@@ -20,8 +20,9 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from ._tables import collect
 from ._lib import (BF16, EXP_AVG, EXP_AVG_SQ, F16, F32, F64, NS_AOL4, NS_AOL4_FP8, NS_CLASSIC5, NS_HAVE_SUMSQ,
-                   STATE_BLOCK, address, check, i64_array, lib, ptr_array)
+                   address, check, i64_array, lib, ptr_array)
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 # element types the cast at the entry of Newton-Schulz accepts (muon.py:760 takes any float dtype)
@@ -206,81 +207,28 @@ def ramped_sizes(sizes: list[int], growth: float = 0.25) -> list[int]:
     return out
 
 
-# ---- tables of many tensors (AdamW, gradient norm, state conversion) --------------------
-# One C-level call per tensor and property: with hundreds of tensors the checks of a call would
-# otherwise take longer than its kernel.
-_dtype_of = Tensor.dtype.__get__
+# ---- many tensors in one call (AdamW, gradient norm, state conversion) -------------------
 _STATE_KINDS = {"exp_avg": EXP_AVG, "exp_avg_sq": EXP_AVG_SQ}
+# masks of element types as _tables.collect takes them
+_T_F32, _T_U8, _T_FLOATS = 1, 8, 7
+_LIKE_FIRST, _SCALES = 0, 1  # sizes of a list: those of the first list, or one per STATE_BLOCK of its elements
+_current_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _dense(t: Tensor) -> bool:
-    """Every element of `t` at a place of its own, without gaps (any order of dimensions)."""
-    at = 1
-    for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz != 1):
-        if stride != at and t.numel() > 0:
-            return False
-        at *= size
-    return True
+def _one_type(mask: int, what: str, name: str) -> int:
+    """Element type code of a list whose tensors must all have one type."""
+    if mask & (mask - 1):
+        raise ValueError(f"{what} needs {name} tensors of one dtype")
+    return mask.bit_length() - 1
 
 
-def state_blocks(numel) -> array:
-    """Scales that 8-bit state of tensors of these sizes has."""
-    return array("q", [-(-n // STATE_BLOCK) for n in numel])
-
-
-class _Tables:
-    """Pointer tables of one call: lists of tensors that are read or written together, element by
-    element in the order of memory. All on one device; written tensors all different."""
-
-    def __init__(self, what: str, first: Sequence[Tensor]):
-        self.what, self.n = what, len(first)
-        self.device_index = first[0].get_device()
-        _require_cuda(first[0], f"every tensor of {what}")
-        self.device = first[0].device
-        self.numel = array("q", map(Tensor.numel, first))
-        self._first, self._strided, self._written, self._n_written = first, False, set(), 0
-
-    def add(self, name: str, tensors: Sequence[Tensor], dtypes=None, numel=None, written: bool = False) -> array:
-        """Table of addresses. `dtypes`: the element types allowed; `numel`: sizes (default: those of
-        the first list, whose memory order the tensors must then share)."""
-        if len(tensors) != self.n:
-            raise ValueError(f"{self.what}: {len(tensors)} {name} tensors for {self.n} tensors")
-        if set(map(Tensor.get_device, tensors)) != {self.device_index}:
-            for t in tensors:
-                _require_cuda(t, f"every {name} tensor of {self.what}")
-            raise ValueError(f"{self.what}: {name} tensors must all be on {self.device}")
-        found = set(map(_dtype_of, tensors))
-        if dtypes is not None and not found <= dtypes:
-            raise ValueError(f"{self.what}: {name} tensors must be {' or '.join(sorted(map(str, dtypes)))}, "
-                             f"got {', '.join(sorted(map(str, found - dtypes)))}")
-        if (self.numel if numel is None else numel) != array("q", map(Tensor.numel, tensors)):
-            raise ValueError(f"{self.what}: a {name} tensor has another number of elements than it must have")
-        if self._strided or not all(map(Tensor.is_contiguous, tensors)):
-            self._check_strides(name, tensors, numel is not None)
-        table = array("Q", map(Tensor.data_ptr, tensors))
-        if written:
-            self._written.update(table)
-            self._n_written += self.n
-            if len(self._written) != self._n_written:
-                self._check_overlap(name)
-        return table
-
-    def _check_strides(self, name, tensors, own_layout: bool) -> None:
-        if tensors is self._first:
-            self._strided = True
-        for t, ref in zip(tensors, self._first):
-            if t.is_contiguous() and (own_layout or ref.is_contiguous()):
-                continue
-            if own_layout or t.stride() != ref.stride() or not _dense(t):
-                raise ValueError(f"{self.what}: {name} tensors must be contiguous, or dense with the strides of the "
-                                 f"tensor they belong to; got shape {tuple(t.shape)}, strides {t.stride()}")
-
-    def _check_overlap(self, name) -> None:
-        """Two written tensors at one address: only tensors without elements may be."""
-        self._written.discard(0)
-        empty = sum(1 for n in self.numel if n == 0)
-        if empty == 0 or len(self._written) < self._n_written - empty * (self._n_written // self.n):
-            raise ValueError(f"{self.what}: a tensor that is written ({name}) appears twice in the call")
+def _call_on(device: int, call, *args) -> None:
+    """A library call with the tensors' device current; the current stream of that device is appended."""
+    if torch.cuda.current_device() == device:
+        check(call(*args, _current_raw_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(call(*args, _current_raw_stream(device)))
 
 
 class CudaBackend:
@@ -615,46 +563,44 @@ class CudaBackend:
             self.launch_groups += 1
 
     # -- AdamW, moments in 32 or 8 bits; gradient norm (adamw.py) --------------------------
-    @staticmethod
-    def _adamw_tables(what, params, grads, masters, steps, grad_scale):
-        """(tables, parameter / gradient / master addresses, steps, dtype codes, factor) of a call."""
-        tab = _Tables(what, params)
-        p = tab.add("parameter", params, written=True)
-        kinds = set(map(_dtype_of, params))
-        code = dtype_code(params[0])
-        if len(kinds) != 1:
-            raise ValueError(f"{what} needs parameters of one dtype, got {', '.join(sorted(map(str, kinds)))}")
-        g = tab.add("gradient", grads, kinds | {torch.float32})
-        if len(set(map(_dtype_of, grads))) != 1:
-            raise ValueError(f"{what} needs gradients of one dtype")
-        w = None if masters is None else tab.add("master", masters, {torch.float32}, written=True)
+    # _tables.collect checks the lists (one device, element types, sizes, memory order, nothing written
+    # twice) and returns their tables of addresses.
+    def _adamw(self, call, what, params, grads, masters, moments, steps, hyper, grad_scale, *seed) -> None:
+        if not params:
+            return
+        lists = [("parameter", params, _T_FLOATS, _LIKE_FIRST, True), ("gradient", grads, _T_FLOATS, _LIKE_FIRST, False)]
+        if masters is not None:
+            lists.append(("master", masters, _T_F32, _LIKE_FIRST, True))
+        device, numel, tables, found, _ = collect(what, (*lists, *moments))
+        code, grad_code = _one_type(found[0], what, "parameter"), _one_type(found[1], what, "gradient")
+        if grad_code != code and grad_code != F32:
+            raise ValueError(f"{what}: gradient tensors must be of the parameters' type or float32")
         if masters is not None and code == F32:
             raise ValueError(f"{what}: float32 parameters have no master weights")
-        steps = array("q", [steps]) * tab.n if isinstance(steps, int) else array("q", steps)
-        if len(steps) != tab.n:
-            raise ValueError(f"{what}: {len(steps)} steps for {tab.n} tensors")
-        if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1
-                                       or grad_scale.get_device() != tab.device_index):
-            raise ValueError(f"{what}: grad_scale must be one float32 value on {tab.device}")
-        return tab, p, g, w, steps, code, dtype_code(grads[0]), None if grad_scale is None else grad_scale.data_ptr()
+        n = len(params)
+        steps = array("q", [steps]) * n if isinstance(steps, int) else array("q", steps)
+        if len(steps) != n:
+            raise ValueError(f"{what}: {len(steps)} steps for {n} tensors")
+        factor = None
+        if grad_scale is not None:
+            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != device:
+                raise ValueError(f"{what}: grad_scale must be one float32 value on cuda:{device}")
+            factor = grad_scale.data_ptr()
+        if _grad_ready:
+            _wait_grads(torch.cuda.current_stream(device), grads)
+        p, g = tables[:2]
+        w, rest = (None, tables[2:]) if masters is None else (tables[2], tables[3:])
+        _call_on(device, call, p, w, g, *rest, numel, address(steps), n, code, grad_code, *hyper, *seed, factor)
+        self.launch_groups += 1
 
     def adamw_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                    exp_avg_sqs: Sequence[Tensor], steps, lr: float, weight_decay: float, betas: tuple[float, float],
                    eps: float, masters=None, grad_scale: Tensor | None = None) -> None:
         """AdamW with float32 moments on tensors of any sizes; one parameter and one gradient dtype."""
-        if not params:
-            return
-        tab, p, g, w, steps, code, g_code, factor = self._adamw_tables("adamw_step", params, grads, masters, steps,
-                                                                       grad_scale)
-        m = tab.add("exp_avg", exp_avgs, {torch.float32}, written=True)
-        v = tab.add("exp_avg_sq", exp_avg_sqs, {torch.float32}, written=True)
-        with torch.cuda.device(tab.device_index):
-            _wait_grads(torch.cuda.current_stream(tab.device), grads)
-            check(lib.muon_b200_adamw(
-                address(p), None if w is None else address(w), address(g), address(m), address(v), address(tab.numel),
-                address(steps), tab.n, code, g_code, lr, weight_decay, betas[0], betas[1], eps, factor,
-                _stream_ptr(tab.device)))
-            self.launch_groups += 1
+        self._adamw(lib.muon_b200_adamw, "adamw_step", params, grads, masters,
+                    (("exp_avg", exp_avgs, _T_F32, _LIKE_FIRST, True),
+                     ("exp_avg_sq", exp_avg_sqs, _T_F32, _LIKE_FIRST, True)),
+                    steps, (lr, weight_decay, betas[0], betas[1], eps), grad_scale)
 
     def adamw8_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg_codes: Sequence[Tensor],
                     exp_avg_scales: Sequence[Tensor], exp_avg_sq_codes: Sequence[Tensor],
@@ -662,42 +608,29 @@ class CudaBackend:
                     betas: tuple[float, float], eps: float, masters=None, grad_scale: Tensor | None = None,
                     seed: int = 0) -> None:
         """AdamW with moments in 8 bits (codes of the parameter's size, one float32 scale per 256)."""
-        if not params:
-            return
-        tab, p, g, w, steps, code, g_code, factor = self._adamw_tables("adamw8_step", params, grads, masters, steps,
-                                                                       grad_scale)
-        blocks = state_blocks(tab.numel)
-        m = tab.add("exp_avg code", exp_avg_codes, {torch.uint8}, written=True)
-        ms = tab.add("exp_avg scale", exp_avg_scales, {torch.float32}, blocks, written=True)
-        v = tab.add("exp_avg_sq code", exp_avg_sq_codes, {torch.uint8}, written=True)
-        vs = tab.add("exp_avg_sq scale", exp_avg_sq_scales, {torch.float32}, blocks, written=True)
-        with torch.cuda.device(tab.device_index):
-            _wait_grads(torch.cuda.current_stream(tab.device), grads)
-            check(lib.muon_b200_adamw8(
-                address(p), None if w is None else address(w), address(g), address(m), address(ms), address(v),
-                address(vs), address(tab.numel), address(steps), tab.n, code, g_code, lr, weight_decay, betas[0],
-                betas[1], eps, seed & 0xFFFFFFFF, factor, _stream_ptr(tab.device)))
-            self.launch_groups += 1
+        self._adamw(lib.muon_b200_adamw8, "adamw8_step", params, grads, masters,
+                    (("exp_avg code", exp_avg_codes, _T_U8, _LIKE_FIRST, True),
+                     ("exp_avg scale", exp_avg_scales, _T_F32, _SCALES, True),
+                     ("exp_avg_sq code", exp_avg_sq_codes, _T_U8, _LIKE_FIRST, True),
+                     ("exp_avg_sq scale", exp_avg_sq_scales, _T_F32, _SCALES, True)),
+                    steps, (lr, weight_decay, betas[0], betas[1], eps), grad_scale, seed & 0xFFFFFFFF)
 
     def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> Tensor:
         """{norm, factor} of all `tensors` together, on their device; with `clip` the tensors are
         multiplied by the factor."""
         what = "clip_grad_norm_" if clip else "grad_norm"
-        tab = _Tables(what, tensors)
-        x = tab.add("gradient", tensors, set(_DTYPE_CODE), written=clip)
-        codes = array("i", [_DTYPE_CODE[d] for d in map(_dtype_of, tensors)])
-        with torch.cuda.device(tab.device_index):
-            _wait_grads(torch.cuda.current_stream(tab.device), tensors)
-            out = torch.empty(2, dtype=torch.float32, device=tab.device)
-            need = lib.muon_b200_grad_norm_scratch_bytes()
-            # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
-            # one stream may be replayed at the same time on two.
-            scratch = (torch.empty(need + 256, dtype=torch.uint8, device=tab.device)
-                       if torch.cuda.is_current_stream_capturing() else self.workspace(tab.device, need, slot=5))
-            call = lib.muon_b200_clip_grads if clip else lib.muon_b200_grad_norm
-            check(call(address(x), address(tab.numel), address(codes), tab.n, max_norm, out.data_ptr(),
-                       self._aligned_ptr(scratch), need, _stream_ptr(tab.device)))
-            self.launch_groups += 1
+        device, numel, tables, _, codes = collect(what, (("gradient", tensors, _T_FLOATS, _LIKE_FIRST, clip),))
+        if _grad_ready:
+            _wait_grads(torch.cuda.current_stream(device), tensors)
+        out = torch.empty(2, dtype=torch.float32, device=tensors[0].device)
+        need = lib.muon_b200_grad_norm_scratch_bytes()
+        # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
+        # one stream may be replayed at the same time on two.
+        scratch = (torch.empty(need + 256, dtype=torch.uint8, device=out.device)
+                   if torch.cuda.is_current_stream_capturing() else self.workspace(out.device, need, slot=5))
+        _call_on(device, lib.muon_b200_clip_grads if clip else lib.muon_b200_grad_norm, tables[0], numel, codes,
+                 len(tensors), max_norm, out.data_ptr(), self._aligned_ptr(scratch), need)
+        self.launch_groups += 1
         return out
 
     def convert_state(self, what: str, values: Sequence[Tensor], codes: Sequence[Tensor], scales: Sequence[Tensor],
@@ -705,18 +638,14 @@ class CudaBackend:
         """Values <-> 8-bit codes and scales, one dtype of values per call."""
         if not codes:
             return
-        tab = _Tables(what, codes)
-        c = tab.add("code", codes, {torch.uint8}, written=to_codes)
-        s = tab.add("scale", scales, {torch.float32}, state_blocks(tab.numel), written=to_codes)
-        x = tab.add("value", values, set(_DTYPE_CODE), written=not to_codes)
-        if len(set(map(_dtype_of, values))) != 1:
-            raise ValueError(f"{what} needs values of one dtype")
+        device, numel, (c, s, x), found, _ = collect(what, (
+            ("code", codes, _T_U8, _LIKE_FIRST, to_codes), ("scale", scales, _T_F32, _SCALES, to_codes),
+            ("value", values, _T_FLOATS, _LIKE_FIRST, not to_codes)))
+        code = _one_type(found[2], what, "value")
         tables = (x, c, s) if to_codes else (c, s, x)
-        call = lib.muon_b200_quantize_state if to_codes else lib.muon_b200_dequantize_state
-        with torch.cuda.device(tab.device_index):
-            check(call(*map(address, tables), address(tab.numel), tab.n, dtype_code(values[0]), _STATE_KINDS[kind],
-                       _stream_ptr(tab.device)))
-            self.launch_groups += 1
+        _call_on(device, lib.muon_b200_quantize_state if to_codes else lib.muon_b200_dequantize_state, *tables, numel,
+                 len(codes), code, _STATE_KINDS[kind])
+        self.launch_groups += 1
 
     # -- functional pieces -------------------------------------------------------------
     def newton_schulz(self, G: Tensor, epsilon: float = 1e-7, mode: str | None = None,

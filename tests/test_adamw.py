@@ -111,9 +111,14 @@ def test_no_cpu_fallback():
             call()
 
 
-def test_tables_tell_dense_from_gapped():
-    from muon_b200.engine import _dense
-    x = torch.zeros(4, 6, 3, 3)
-    assert _dense(x) and _dense(x.to(memory_format=torch.channels_last)) and _dense(x.permute(3, 1, 0, 2))
-    assert _dense(torch.zeros(5, 1).t()) and _dense(torch.zeros(0, 7)) and _dense(torch.zeros(()))
-    assert not _dense(x[:, ::2]) and not _dense(torch.zeros(4).expand(3, 4)) and not _dense(torch.zeros(4, 8)[:, :4])
+def test_pointer_tables_refuse_what_is_no_cuda_tensor():
+    from muon_b200._tables import collect
+    with pytest.raises(RuntimeError, match="every gradient tensor of grad_norm .* no CPU implementation"):
+        collect("grad_norm", (("gradient", [torch.zeros(3)], 7, 0, False),))
+    for bad in ([1], [None], [[torch.zeros(1)]]):
+        with pytest.raises(TypeError, match="is no tensor"):
+            collect("grad_norm", (("gradient", bad, 7, 0, False),))
+    with pytest.raises(TypeError):
+        collect("grad_norm", (("gradient", 5, 7, 0, False),))
+    device, numel, tables, found, codes = collect("grad_norm", (("gradient", [], 7, 0, False),))
+    assert (device, numel, tables, found, codes) == (-1, b"", (b"",), (0,), b"")

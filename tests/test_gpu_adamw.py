@@ -503,12 +503,15 @@ def test_refusals(mb):
         (lambda: mb.adamw_step([p[0]], [f()], [p[0]], [f()], 1), ValueError, "twice"),
         (lambda: mb.adamw8_step([f()], [f()], [f()], [f(1)], [f()], [f(1)], 1), ValueError, "uint8"),
         (lambda: mb.adamw8_step([f()], [f()], [f(dtype=torch.uint8)], [f(2)], [f(dtype=torch.uint8)], [f(1)], 1), ValueError,
-         "exp_avg scale tensor has another number"),
+         "exp_avg scale tensor 0 has another number"),
         (lambda: mb.adamw8_step([f()], [f()], [f(dtype=torch.uint8)], [f(1)], [f(dtype=torch.uint8)], [f(1)], 1, eps=0.0),
          mb.MuonB200Error, "eps"),
         (lambda: mb.quantize_state([f()], "momentum"), ValueError, "kind"),
         (lambda: mb.dequantize_state([f(dtype=torch.uint8)], [f(1)], "exp_avg", dtype=torch.float64), ValueError, "float64"),
         (lambda: mb.clip_grad_norm_([p[0], p[0]], 1.0), ValueError, "twice"),
+        (lambda: mb.clip_grad_norm_([p[0][:6], f(), p[0][5:]], 1.0), ValueError, "twice"),
+        (lambda: mb.adamw_step([p[0][:6]], [f(6)], [p[0][4:]], [f(6)], 1), ValueError, "twice"),
+        (lambda: mb.adamw_step([f()], [None], [f()], [f()], 1), TypeError, "is no tensor"),
         (lambda: mb.clip_grad_norm_([f()], -1.0), mb.MuonB200Error, "max_norm"),
         (lambda: mb.clip_grad_norm_([f()], float("nan")), mb.MuonB200Error, "max_norm"),
         (lambda: mb.grad_norm([f(dtype=torch.int32)]), ValueError, "int32"),
