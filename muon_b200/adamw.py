@@ -15,6 +15,7 @@ import torch
 from torch import Tensor
 
 from ._lib import STATE_BLOCK
+from ._tables import gradients
 from .engine import _STATE_KINDS, get_backend
 
 
@@ -55,12 +56,9 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg_codes
 
 def _gradients(tensors) -> list[Tensor]:
     """The gradients of parameters (those that have one), or the tensors themselves."""
-    if isinstance(tensors, Tensor):
-        tensors = [tensors]
-    return [g for g in (t.grad if isinstance(t, torch.nn.Parameter) else t for t in tensors) if g is not None]
+    return gradients([tensors] if isinstance(tensors, Tensor) else tensors)
 
 
-@torch.no_grad()
 def grad_norm(tensors, max_norm: float = math.inf) -> tuple[Tensor, Tensor]:
     """2-norm of all elements of ``tensors`` (gradients, or parameters, meaning their ``.grad``)
     together, and the factor min(1, max_norm / (norm + 1e-6)) that brings it down to ``max_norm``: two
@@ -71,11 +69,9 @@ def grad_norm(tensors, max_norm: float = math.inf) -> tuple[Tensor, Tensor]:
     tensors = _gradients(tensors)
     if not tensors:
         return torch.zeros(()), torch.ones(())
-    out = get_backend().grad_norm(tensors, max_norm, clip=False)
-    return out[0], out[1]
+    return get_backend().grad_norm(tensors, max_norm, clip=False).unbind()
 
 
-@torch.no_grad()
 def clip_grad_norm_(tensors, max_norm: float) -> Tensor:
     """Scale gradients in place so that their 2-norm together is at most ``max_norm`` (as
     ``torch.nn.utils.clip_grad_norm_`` does): gradients, or parameters, meaning their ``.grad``. Returns the norm
@@ -91,7 +87,6 @@ def _check_kind(kind: str) -> None:
         raise ValueError(f"unknown kind of state {kind!r}; expected one of {sorted(_STATE_KINDS)}")
 
 
-@torch.no_grad()
 def quantize_state(tensors: Sequence[Tensor], kind: str, *, codes: Sequence[Tensor] | None = None,
                    scales: Sequence[Tensor] | None = None) -> tuple[Sequence[Tensor], Sequence[Tensor]]:
     """Moments (``kind``: "exp_avg" or "exp_avg_sq") as 8-bit codes and scales, rounded to nearest, into
@@ -105,7 +100,6 @@ def quantize_state(tensors: Sequence[Tensor], kind: str, *, codes: Sequence[Tens
     return codes, scales
 
 
-@torch.no_grad()
 def dequantize_state(codes: Sequence[Tensor], scales: Sequence[Tensor], kind: str, *,
                      dtype: torch.dtype = torch.float32, out: Sequence[Tensor] | None = None) -> Sequence[Tensor]:
     """What the codes and scales of 8-bit moments stand for, as tensors of ``dtype``, or in ``out``."""

@@ -10,6 +10,7 @@
 #include <cuda_fp8.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <type_traits>
 
 namespace mb {
@@ -67,25 +68,32 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 template <typename T, int N>
 struct Raw {  // the words of N elements, as loaded
   static constexpr int kWords = N * (int)sizeof(T) / 16;
-  static_assert(kWords == 1 || kWords == 2, "16 or 32 bytes");
+  static_assert(kWords == 1 || kWords % 2 == 0, "16 bytes or pieces of 32");
   uint4 w[kWords];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kWords == 1)
-      w[0] = __ldcs(reinterpret_cast<const uint4*>(p));
-    else
+  __device__ __forceinline__ void load(const T* p) {  // streaming, of one use
+    if constexpr (kWords == 1) w[0] = __ldcs(reinterpret_cast<const uint4*>(p));
+    else load_pairs(p);
+  }
+  __device__ __forceinline__ void load_pairs(const T* p) {
+#pragma unroll
+    for (int k = 0; k + 1 < kWords; k += 2)
       asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(w[0].x), "=r"(w[0].y), "=r"(w[0].z), "=r"(w[0].w), "=r"(w[1].x), "=r"(w[1].y), "=r"(w[1].z),
-                     "=r"(w[1].w)
-                   : "l"(p)
+                   : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w), "=r"(w[k + 1].x), "=r"(w[k + 1].y),
+                     "=r"(w[k + 1].z), "=r"(w[k + 1].w)
+                   : "l"(reinterpret_cast<const uint4*>(p) + k)
                    : "memory");
   }
   __device__ __forceinline__ void store(T* p) const {
-    if constexpr (kWords == 1)
+    if constexpr (kWords == 1) {
       __stcs(reinterpret_cast<uint4*>(p), w[0]);
-    else
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0].x), "r"(w[0].y),
-                   "r"(w[0].z), "r"(w[0].w), "r"(w[1].x), "r"(w[1].y), "r"(w[1].z), "r"(w[1].w)
-                   : "memory");
+    } else {
+#pragma unroll
+      for (int k = 0; k + 1 < kWords; k += 2)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint4*>(p) + k),
+                     "r"(w[k].x), "r"(w[k].y), "r"(w[k].z), "r"(w[k].w), "r"(w[k + 1].x), "r"(w[k + 1].y),
+                     "r"(w[k + 1].z), "r"(w[k + 1].w)
+                     : "memory");
+    }
   }
   __device__ __forceinline__ void unpack(float (&v)[N]) const {
 #pragma unroll
@@ -152,6 +160,10 @@ __device__ __forceinline__ int find_tensor(const S& start, int count, int chunk)
   return lo;
 }
 
+// Tensors that start anywhere are handled in aligned pieces from their `head` on, where the lists of a
+// tensor are all aligned at one element (as in tensors packed one behind the other).
+constexpr unsigned char kNoHead = 255;
+
 struct AdamWConsts {
   float b1, w1, b2, w2;  // float(beta), float(1 - beta)
   float eps, decay;      // decay = float(1 - lr * weight_decay)
@@ -193,7 +205,7 @@ struct AdamW32Args {
   long long numel[CAP];
   float step[CAP], rs[CAP];
   int start[CAP + 1];
-  unsigned char vec_ok[CAP];
+  unsigned char head[CAP];  // elements before the first that is aligned in every list; kNoHead: none is
 };
 
 template <typename P>
@@ -209,7 +221,9 @@ adamw32_kernel(const __grid_constant__ AdamW32Args<CAP> a) {
   float f;
   if (!read_factor(a.c.grad_scale, f)) return;
   const int t = find_tensor(a.start, a.c.count, (int)blockIdx.x);
-  const long long base = (long long)((int)blockIdx.x - a.start[t]) * kChunk32<P>;
+  const int head = a.head[t] == kNoHead ? 0 : a.head[t];
+  const int chunk = (int)blockIdx.x - a.start[t];
+  const long long base = (long long)chunk * kChunk32<P> + head;
   const long long left = a.numel[t] - base;
   P* p = static_cast<P*>(a.p[t]) + base;
   float* w = MASTER ? a.w[t] + base : nullptr;
@@ -225,7 +239,7 @@ adamw32_kernel(const __grid_constant__ AdamW32Args<CAP> a) {
     pj = moved(pj, mj, vj, c.decay, step, rs, c.eps);
   };
   int done = 0;  // elements of the chunk that the vector loop covers
-  if (a.vec_ok[t]) {
+  if (a.head[t] != kNoHead) {
     done = left >= kChunk32<P> ? kChunk32<P> : (int)left / V * V;
 #pragma unroll 2
     for (int i = threadIdx.x * V; i < done; i += kThreads * V) {
@@ -257,15 +271,17 @@ adamw32_kernel(const __grid_constant__ AdamW32Args<CAP> a) {
       rp.store(p + i);
     }
   }
-  const int end = left < kChunk32<P> ? (int)left : kChunk32<P>;
-  for (int i = done + threadIdx.x; i < end; i += kThreads) {
+  const auto single = [&](int i) {
     float pj = MASTER ? w[i] : to_float<P>(p[i]), mj = m[i], vj = v[i];
     one(pj, to_float<G>(g[i]), mj, vj);
     m[i] = mj;
     v[i] = vj;
     if (MASTER) w[i] = pj;
     p[i] = from_float<P>(pj);
-  }
+  };
+  const int end = left < kChunk32<P> ? (int)left : kChunk32<P>;
+  for (int i = done + threadIdx.x; i < end; i += kThreads) single(i);
+  if (chunk == 0 && (int)threadIdx.x < head) single((int)threadIdx.x - head);
 }
 
 // ---------------------------------------------------------------------------
@@ -553,7 +569,7 @@ constexpr int kStages8 = 3;
 template <typename P, typename G, bool MASTER>
 constexpr int kShared8 = kWarps * kStages8 * Stage8<P, G, MASTER>::kBytes;
 
-// A warp takes `per_warp` consecutive blocks (at most 32). Each lane copies its share of a block to shared
+// A warp takes `per_warp` consecutive blocks (at most 32: a lane holds the scales of one). Each lane copies its share of a block to shared
 // memory kStages8 - 1 blocks ahead, asynchronously, and later reads back what it copied itself, so no
 // barrier is needed and the loads in flight hold no registers. Scales are read and written once
 // per task, lane k's for block k.
@@ -657,17 +673,19 @@ struct ConvertArgs {
   uint32_t half;  // half a code (2^19), added before the cut: to nearest
 };
 
-template <typename T, int KIND, bool TO_CODES, int CAP>
+template <typename T, int KIND, int CAP>
 __global__ void __launch_bounds__(kThreads)
-convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
+quantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
   const int t = find_tensor(a.start, a.count, (int)blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long numel = a.numel[t];
   const long long blocks = (numel + kStateBlock - 1) / kStateBlock;
-  T* x = static_cast<T*>(a.x[t]);
+  const T* x = static_cast<const T*>(a.x[t]);
   uint8_t* codes = a.codes[t];
-  float* scales = a.scales[t];
   const long long first = (long long)((int)blockIdx.x - a.start[t]) * kBlocksPerChunk + warp;
+  // half a code is added before the cut (an argument, because with the constant in its place the
+  // compiler's code saturated every value)
+  const uint32_t r[8] = {a.half, a.half, a.half, a.half, a.half, a.half, a.half, a.half};
 #pragma unroll
   for (int k = 0; k < kBlocksPerWarp; ++k) {
     const long long b = first + (long long)k * kWarps;
@@ -676,48 +694,82 @@ convert_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
     const long long at = base + lane * 8;
     const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
     float2 xj[4];
-    if constexpr (TO_CODES) {
-      if (vec) {
-        Raw<T, 8> rx;
-        rx.load(x + at);
-        rx.unpack(xj);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const long long i = base + lane + 32 * j;
-          (j & 1 ? xj[j / 2].y : xj[j / 2].x) = i < numel ? to_float<T>(x[i]) : 0.f;
-        }
-      }
-      const float amax = warp_max(amax_bits(xj)), inv = block_factor<KIND>(amax);
-      if (lane == 0) scales[b] = block_scale<KIND>(amax);
-      // (an argument, because with the constant in its place the compiler's code saturated every value)
-      const uint32_t r[8] = {a.half, a.half, a.half, a.half, a.half, a.half, a.half, a.half};
-      const uint2 c = encode8<KIND>(xj, inv, r);
-      if (vec) {
-        __stcs(reinterpret_cast<uint2*>(codes + at), c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const long long i = base + lane + 32 * j;
-          if (i < numel) codes[i] = byte_of(c, j);
-        }
-      }
+    if (vec) {
+      Raw<T, 8> rx;
+      rx.load(x + at);
+      rx.unpack(xj);
     } else {
-      const float scale = scales[b];
-      if (vec) {
-        decode8<KIND>(__ldcs(reinterpret_cast<const uint2*>(codes + at)), scale, xj);
-        Raw<T, 8> rx;
-        rx.pack(xj);
-        rx.store(x + at);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const long long i = base + lane + 32 * j;
-          if (i < numel) x[i] = from_float<T>(decode1<KIND>(codes[i], scale));
-        }
+      for (int j = 0; j < 8; ++j) {
+        const long long i = base + lane + 32 * j;
+        (j & 1 ? xj[j / 2].y : xj[j / 2].x) = i < numel ? to_float<T>(x[i]) : 0.f;
+      }
+    }
+    const float amax = warp_max(amax_bits(xj)), inv = block_factor<KIND>(amax);
+    if (lane == 0) a.scales[t][b] = block_scale<KIND>(amax);
+    const uint2 c = encode8<KIND>(xj, inv, r);
+    if (vec) {
+      __stcs(reinterpret_cast<uint2*>(codes + at), c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const long long i = base + lane + 32 * j;
+        if (i < numel) codes[i] = byte_of(c, j);
       }
     }
   }
+}
+
+// A warp expands four consecutive blocks: 16 codes a lane from two blocks at a time, so that codes are
+// read and values written 16 bytes and more to a lane.
+template <typename T, int KIND, int CAP>
+__global__ void __launch_bounds__(kThreads)
+dequantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
+  const int t = find_tensor(a.start, a.count, (int)blockIdx.x);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long numel = a.numel[t];
+  T* x = static_cast<T*>(a.x[t]);
+  const uint8_t* codes = a.codes[t];
+  const float* scales = a.scales[t];
+  const long long b0 = ((long long)((int)blockIdx.x - a.start[t]) * kWarps + warp) * kBlocksPerWarp;
+  const long long base = b0 * kStateBlock;
+  if (base >= numel) return;
+  if (a.vec_ok[t]) {
+    constexpr int kPieces = kBlocksPerWarp / 2;
+    uint4 c[kPieces];
+    float scale[kPieces];
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const long long at = base + 2 * k * kStateBlock + 16 * lane;
+      if (at >= numel) continue;
+      scale[k] = scales[b0 + 2 * k + (lane >> 4)];
+      if (at + 16 <= numel) c[k] = __ldcs(reinterpret_cast<const uint4*>(codes + at));
+    }
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const long long at = base + 2 * k * kStateBlock + 16 * lane;
+      if (at + 16 <= numel) {
+        float2 lo[4], hi[4], all[8];
+        decode8<KIND>(make_uint2(c[k].x, c[k].y), scale[k], lo);
+        decode8<KIND>(make_uint2(c[k].z, c[k].w), scale[k], hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          all[j] = lo[j];
+          all[4 + j] = hi[j];
+        }
+        Raw<T, 16> rx;
+        rx.pack(all);
+        rx.store(x + at);
+      } else {
+        for (long long i = at; i < numel; ++i) x[i] = from_float<T>(decode1<KIND>(codes[i], scale[k]));
+      }
+    }
+    return;
+  }
+  const int n = (int)min(numel - base, (long long)kBlocksPerWarp * kStateBlock);
+#pragma unroll 8
+  for (int i = lane; i < n; i += 32)
+    x[base + i] = from_float<T>(decode1<KIND>(codes[base + i], scales[b0 + i / kStateBlock]));
 }
 
 // ---------------------------------------------------------------------------
@@ -732,49 +784,66 @@ struct NormArgs {
   long long numel[CAP];
   int start[CAP + 1];
   unsigned char dtype[CAP];
-  unsigned char vec_ok[CAP];
+  unsigned char head[CAP];  // elements before the first that is aligned
   int count, chunks;
   double* partials;
 };
 
+// A thread takes 32 bytes at a time, kNormIters times in a chunk.
 constexpr int kNormIters = 4;
-constexpr int kNormChunk = kThreads * 8 * kNormIters;
+constexpr int kNormBlocksPerSm = 4;
+template <typename T>
+constexpr int kNormVec = 32 / (int)sizeof(T);
+template <typename T>
+constexpr int kNormChunk = kThreads * kNormIters * kNormVec<T>;
 
-__device__ __forceinline__ double squares(const float (&x)[8]) {
-  float s = 0.f;
+template <int N>
+__device__ __forceinline__ double squares(const float (&x)[N]) {
+  float s[2] = {0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], s);
-  if (s < 3e38f && s > 1e-30f) return (double)s;
+  for (int j = 0; j < N; ++j) s[j & 1] = fmaf(x[j], x[j], s[j & 1]);
+  const float sum = s[0] + s[1];
+  if (sum < 3e38f && sum > 1e-30f) return (double)sum;
   uint32_t any = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) any |= __float_as_uint(x[j]) << 1;
+  for (int j = 0; j < N; ++j) any |= __float_as_uint(x[j]) << 1;
   if (any == 0) return 0.0;
   double d = 0.0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) d += (double)x[j] * (double)x[j];
+  for (int j = 0; j < N; ++j) d += (double)x[j] * (double)x[j];
   return d;
 }
 
+// A chunk of a tensor: `head` elements behind the tensor's start, of which the first chunk also takes the head.
 template <typename T>
-__device__ __forceinline__ double chunk_squares(const T* x, long long left, bool vec) {
+__device__ __forceinline__ double chunk_squares(const T* x, int chunk, int head, long long numel) {
+  constexpr int V = kNormVec<T>, kChunk = kNormChunk<T>;
   double acc = 0.0;
-  int done = 0;
-  const int end = left < kNormChunk ? (int)left : kNormChunk;
-  if (vec) {
-    done = end / 8 * 8;
+  const long long base = (long long)chunk * kChunk + head;
+  const int end = (int)min(numel - base, (long long)kChunk), done = end / V * V;
+  x += base;
+  if (end == kChunk) {
+    Raw<T, V> rx[kNormIters];  // all loads before the sums, whose rare branch they could not cross
+#pragma unroll
+    for (int k = 0; k < kNormIters; ++k) rx[k].load(x + (k * kThreads + threadIdx.x) * V);
 #pragma unroll
     for (int k = 0; k < kNormIters; ++k) {
-      const int i = (k * kThreads + threadIdx.x) * 8;
-      if (i < done) {
-        Raw<T, 8> rx;
-        rx.load(x + i);
-        float v[8];
-        rx.unpack(v);
-        acc += squares(v);
-      }
+      float v[V];
+      rx[k].unpack(v);
+      acc += squares(v);
+    }
+  } else {
+    for (int i = threadIdx.x * V; i < done; i += kThreads * V) {
+      Raw<T, V> rx;
+      rx.load(x + i);
+      float v[V];
+      rx.unpack(v);
+      acc += squares(v);
     }
   }
-  for (int i = done + threadIdx.x; i < end; i += kThreads) {
+  int i = done + threadIdx.x;  // fewer than V behind the last whole piece, and the head
+  if (i >= end) i = chunk == 0 && (int)threadIdx.x >= kThreads - head ? (int)threadIdx.x - kThreads : end;
+  if (i < end) {
     const double v = (double)to_float<T>(x[i]);
     acc += v * v;
   }
@@ -794,18 +863,17 @@ __device__ __forceinline__ double block_sum(double v, double (&warps)[kWarps]) {
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kNormBlocksPerSm)
 norm_partial_kernel(const __grid_constant__ NormArgs<CAP> a) {
   __shared__ double warps[kWarps];
   double acc = 0.0;
   for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
     const int t = find_tensor(a.start, a.count, chunk);
-    const long long base = (long long)(chunk - a.start[t]) * kNormChunk;
-    const long long left = a.numel[t] - base;
-    const bool vec = a.vec_ok[t] != 0;
-    if (a.dtype[t] == DT_F32) acc += chunk_squares(static_cast<const float*>(a.x[t]) + base, left, vec);
-    else if (a.dtype[t] == DT_BF16) acc += chunk_squares(static_cast<const __nv_bfloat16*>(a.x[t]) + base, left, vec);
-    else acc += chunk_squares(static_cast<const __half*>(a.x[t]) + base, left, vec);
+    const int k = chunk - a.start[t], head = a.head[t];
+    const long long n = a.numel[t];
+    if (a.dtype[t] == DT_F32) acc += chunk_squares(static_cast<const float*>(a.x[t]), k, head, n);
+    else if (a.dtype[t] == DT_BF16) acc += chunk_squares(static_cast<const __nv_bfloat16*>(a.x[t]), k, head, n);
+    else acc += chunk_squares(static_cast<const __half*>(a.x[t]), k, head, n);
   }
   acc = block_sum(acc, warps);
   if (threadIdx.x == 0) a.partials[blockIdx.x] = acc;
@@ -831,27 +899,25 @@ norm_finish_kernel(const double* partials, int n, float max_norm, float* out2) {
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_chunk(T* x, long long left, bool vec, float f) {
-  int done = 0;
-  const int end = left < kNormChunk ? (int)left : kNormChunk;
-  if (vec) {
-    done = end / 8 * 8;
+__device__ __forceinline__ void scale_chunk(T* x, int chunk, int head, long long numel, float f) {
+  constexpr int V = kNormVec<T>, kChunk = kNormChunk<T>;
+  const long long base = (long long)chunk * kChunk + head;
+  const int end = (int)min(numel - base, (long long)kChunk), done = end / V * V;
+  x += base;
+#pragma unroll 2
+  for (int i = threadIdx.x * V; i < done; i += kThreads * V) {
+    Raw<T, V> rx;
+    rx.load(x + i);
+    float v[V];
+    rx.unpack(v);
 #pragma unroll
-    for (int k = 0; k < kNormIters; ++k) {
-      const int i = (k * kThreads + threadIdx.x) * 8;
-      if (i < done) {
-        Raw<T, 8> rx;
-        rx.load(x + i);
-        float v[8];
-        rx.unpack(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= f;
-        rx.pack(v);
-        rx.store(x + i);
-      }
-    }
+    for (int j = 0; j < V; ++j) v[j] *= f;
+    rx.pack(v);
+    rx.store(x + i);
   }
-  for (int i = done + threadIdx.x; i < end; i += kThreads) x[i] = from_float<T>(to_float<T>(x[i]) * f);
+  int i = done + threadIdx.x;
+  if (i >= end) i = chunk == 0 && (int)threadIdx.x >= kThreads - head ? (int)threadIdx.x - kThreads : end;
+  if (i < end) x[i] = from_float<T>(to_float<T>(x[i]) * f);
 }
 
 template <int CAP>
@@ -865,14 +931,13 @@ clip_kernel(const __grid_constant__ NormArgs<CAP> a, int partials, float max_nor
   }
   const float f = r.y;
   if (f == 1.f) return;  // nothing to clip: x * 1 is x
-  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+  for (int chunk = a.chunks - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
     const int t = find_tensor(a.start, a.count, chunk);
-    const long long base = (long long)(chunk - a.start[t]) * kNormChunk;
-    const long long left = a.numel[t] - base;
-    const bool vec = a.vec_ok[t] != 0;
-    if (a.dtype[t] == DT_F32) scale_chunk(static_cast<float*>(a.x[t]) + base, left, vec, f);
-    else if (a.dtype[t] == DT_BF16) scale_chunk(static_cast<__nv_bfloat16*>(a.x[t]) + base, left, vec, f);
-    else scale_chunk(static_cast<__half*>(a.x[t]) + base, left, vec, f);
+    const int k = chunk - a.start[t], head = a.head[t];
+    const long long n = a.numel[t];
+    if (a.dtype[t] == DT_F32) scale_chunk(static_cast<float*>(a.x[t]), k, head, n, f);
+    else if (a.dtype[t] == DT_BF16) scale_chunk(static_cast<__nv_bfloat16*>(a.x[t]), k, head, n, f);
+    else scale_chunk(static_cast<__half*>(a.x[t]), k, head, n, f);
   }
 }
 
@@ -882,6 +947,35 @@ clip_kernel(const __grid_constant__ NormArgs<CAP> a, int partials, float max_nor
 inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 inline int elem_bytes(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
+struct BiasCorrection {  // lr / (1 - b1^t) and 1 / sqrt(1 - b2^t); most tensors of a call share t
+  int64_t t = 0;
+  float step = 0.f, rs = 0.f;
+  void set(const AdamWCall& c, int64_t now) {
+    if (now == t) return;
+    t = now;
+    step = (float)(c.lr / (1.0 - std::pow(c.beta1, (double)t)));
+    rs = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)t)));
+  }
+};
+
+struct ListStart {
+  const void* p;
+  size_t bytes;  // of an element
+};
+// The first element, under N, at which all lists are aligned to N elements; kNoHead: there is none.
+template <int N>
+int common_head(std::initializer_list<ListStart> lists) {
+  int head = -1;
+  for (const ListStart& l : lists) {
+    if (!l.p) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(l.p) / l.bytes;  // (aligned to its elements)
+    const int h = (int)((N - at % N) % N);
+    if (head >= 0 && h != head) return kNoHead;
+    head = h;
+  }
+  return head < 0 ? 0 : head;
+}
+
 // Adds `chunks` to the running total of a launch; false when the launch must go out first.
 inline bool fits(int total, int64_t chunks) { return chunks <= (int64_t)INT32_MAX - total; }
 
@@ -889,12 +983,21 @@ template <typename P, typename G, bool MASTER, int CAP>
 int adamw32_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
   AdamW32Args<CAP> a;
   a.c = consts;
+  BiasCorrection bias;
   const double bytes = (MASTER ? sizeof(P) + 8.0 : 2.0 * sizeof(P)) + sizeof(G) + 16.0;
   int n = 0;
   double elems = 0;
   a.start[0] = 0;
   for (int i = 0; i <= c.count; ++i) {
-    const int64_t chunks = i < c.count ? (c.numel[i] + kChunk32<P> - 1) / kChunk32<P> : 0;
+    constexpr int V = kVec32<P>;
+    int head = 0;
+    int64_t chunks = 0;
+    if (i < c.count && c.numel[i] > 0) {
+      head = common_head<V>({{c.param[i], sizeof(P)}, {c.grad[i], sizeof(G)}, {c.exp_avg[i], 4}, {c.exp_avg_sq[i], 4},
+                             {MASTER ? c.master[i] : nullptr, 4}});
+      if (head >= c.numel[i]) head = kNoHead;
+      chunks = (c.numel[i] - (head == kNoHead ? 0 : head) + kChunk32<P> - 1) / kChunk32<P>;
+    }
     if (i == c.count || n == CAP || !fits(a.start[n], chunks)) {
       if (n > 0) {
         a.c.count = n;
@@ -912,10 +1015,10 @@ int adamw32_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t s
     a.m[n] = static_cast<float*>(c.exp_avg[i]);
     a.v[n] = static_cast<float*>(c.exp_avg_sq[i]);
     a.numel[n] = c.numel[i];
-    a.step[n] = (float)(c.lr / (1.0 - std::pow(c.beta1, (double)c.steps[i])));
-    a.rs[n] = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)c.steps[i])));
-    a.vec_ok[n] = aligned(a.p[n], kVec32<P> * sizeof(P)) && aligned(a.g[n], kVec32<P> * sizeof(G)) &&
-                  aligned(a.m[n], kVec32<P> * 4) && aligned(a.v[n], kVec32<P> * 4) && aligned(a.w[n], kVec32<P> * 4);
+    bias.set(c, c.steps[i]);
+    a.step[n] = bias.step;
+    a.rs[n] = bias.rs;
+    a.head[n] = (unsigned char)head;
     a.start[n + 1] = a.start[n] + (int)chunks;
     elems += (double)c.numel[i];
     ++n;
@@ -923,19 +1026,21 @@ int adamw32_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t s
   return OK;
 }
 
-// Blocks per warp: long tasks keep the pipeline of copies full, short ones leave a shorter tail at the end
-// of the launch and of each tensor. 16 rounds of resident warps where there is work for them: 128
-// filters, 47 million float32 weights, take 183, 174, 164, 160, 172 us with 2, 4, 8, 16, 32 rounds.
+// Blocks per warp: long tasks keep the pipeline of copies full, short ones leave a shorter tail. As many as
+// make one round of resident warps, at most kMostPerWarp: two layers of 436M bf16 weights take 877, 723,
+// 677, 658, 664, 679 us with 2, 4, 6, 8, 12, 16 blocks a warp, 150 tensors of 72 thousand float32
+// weights 38 us with one and 28 with eight, 90 of 53 thousand 16.6 with one, 12.4 with six, 15.1 with eight.
+constexpr int kMostPerWarp = 8;
 inline int blocks_per_warp(double blocks, int sms) {
-  const double tasks = 16.0 * sms * kBlocksPerSm8 * kWarps;
-  const int per = (int)(blocks / tasks);
-  return per < 1 ? 1 : per > 32 ? 32 : per;
+  const int per = (int)std::ceil(blocks / ((double)sms * kBlocksPerSm8 * kWarps));
+  return per < 1 ? 1 : per > kMostPerWarp ? kMostPerWarp : per;
 }
 
 template <typename P, typename G, bool MASTER, int CAP>
 int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
   AdamW8Args<CAP> a;
   a.c = consts;
+  BiasCorrection bias;
   const double bytes = (MASTER ? sizeof(P) + 8.0 : 2.0 * sizeof(P)) + sizeof(G) + 4.0 + 16.0 / kStateBlock;
   constexpr int kShared = kShared8<P, G, MASTER>;
   MB_CUDA_CHECK(cudaFuncSetAttribute(adamw8_kernel<P, G, MASTER, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
@@ -969,8 +1074,9 @@ int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t st
     a.v[n] = static_cast<uint8_t*>(c.exp_avg_sq[i]);
     a.vs[n] = static_cast<float*>(c.exp_avg_sq_scale[i]);
     a.numel[n] = c.numel[i];
-    a.step[n] = (float)(c.lr / (1.0 - std::pow(c.beta1, (double)c.steps[i])));
-    a.rs[n] = (float)(1.0 / std::sqrt(1.0 - std::pow(c.beta2, (double)c.steps[i])));
+    bias.set(c, c.steps[i]);
+    a.step[n] = bias.step;
+    a.rs[n] = bias.rs;
     a.key[n] = random_key(c.seed, c.steps[i]);
     a.vec_ok[n] = aligned(a.p[n], 8 * sizeof(P)) && aligned(a.g[n], 8 * sizeof(G)) && aligned(a.m[n], 8) &&
                   aligned(a.v[n], 8) && aligned(a.w[n], 32);
@@ -981,12 +1087,18 @@ int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t st
   return OK;
 }
 
-constexpr int kCapAdamW32 = 512, kCapAdamW8 = 384, kCapConvert = 512, kCapNorm = 1024;
+// Tensors per launch: as many as 32764 bytes of arguments hold, or, for calls with few, a table that takes the
+// host less time to hand over (a conversion of 25 tensors returns after 7.5 instead of 10.4 us).
+constexpr int kCapFew = 64, kCapAdamW32 = 512, kCapAdamW8 = 384, kCapConvert = 512, kCapNorm = 1024;
 
 template <typename P, typename G, bool MASTER>
 int adamw_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t stream) {
-  if (c.exp_avg_scale) return adamw8_launch<P, G, MASTER, kCapAdamW8>(c, consts, stream);
-  return adamw32_launch<P, G, MASTER, kCapAdamW32>(c, consts, stream);
+  const bool few = c.count <= kCapFew;
+  if (c.exp_avg_scale)
+    return few ? adamw8_launch<P, G, MASTER, kCapFew>(c, consts, stream)
+               : adamw8_launch<P, G, MASTER, kCapAdamW8>(c, consts, stream);
+  return few ? adamw32_launch<P, G, MASTER, kCapFew>(c, consts, stream)
+             : adamw32_launch<P, G, MASTER, kCapAdamW32>(c, consts, stream);
 }
 
 template <typename P, typename G>
@@ -1004,7 +1116,14 @@ int for_each_norm_table(void* const* tensors, const int64_t* numel, const int* d
   double bytes = 0;
   a.start[0] = 0;
   for (int i = 0; i <= count; ++i) {
-    const int64_t chunks = i < count ? (numel[i] + kNormChunk - 1) / kNormChunk : 0;
+    int head = 0;
+    int64_t chunks = 0;
+    if (i < count && numel[i] > 0) {
+      const int size = elem_bytes(dtypes[i]), chunk = size == 4 ? kNormChunk<float> : kNormChunk<__half>;
+      head = (int)((32 - reinterpret_cast<uintptr_t>(tensors[i]) % 32) % 32) / size;
+      if (head > numel[i]) head = (int)numel[i];
+      chunks = numel[i] == head ? 1 : (numel[i] - head + chunk - 1) / chunk;
+    }
     if (i == count || n == CAP || !fits(a.start[n], chunks)) {
       if (n > 0) {
         a.count = n;
@@ -1019,7 +1138,7 @@ int for_each_norm_table(void* const* tensors, const int64_t* numel, const int* d
     a.x[n] = tensors[i];
     a.numel[n] = numel[i];
     a.dtype[n] = (unsigned char)dtypes[i];
-    a.vec_ok[n] = aligned(tensors[i], 8 * elem_bytes(dtypes[i]));
+    a.head[n] = (unsigned char)head;
     a.start[n + 1] = a.start[n] + (int)chunks;
     bytes += (double)numel[i] * elem_bytes(dtypes[i]);
     ++n;
@@ -1027,7 +1146,6 @@ int for_each_norm_table(void* const* tensors, const int64_t* numel, const int* d
   return OK;
 }
 
-constexpr int kNormBlocksPerSm = 8;
 constexpr int kNormTables = 64;  // launches of the norm kernel per call: 64 * 1024 tensors
 
 int norm_grid(int chunks, int* grid) {
@@ -1038,18 +1156,19 @@ int norm_grid(int chunks, int* grid) {
   return OK;
 }
 
+template <int CAP>
 int norm_partials(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double* partials,
                   int* n_partials, cudaStream_t stream) {
   int used = 0, tables = 0;
-  const int rc = for_each_norm_table<kCapNorm>(
-      tensors, numel, dtypes, count, partials, [&](NormArgs<kCapNorm>& a, double bytes) -> int {
+  const int rc = for_each_norm_table<CAP>(
+      tensors, numel, dtypes, count, partials, [&](NormArgs<CAP>& a, double bytes) -> int {
         int grid = 0;
         const int rc = norm_grid(a.chunks, &grid);
         if (rc != OK) return rc;
         if (++tables > kNormTables) return set_error(ERR_UNSUPPORTED, "gradient norm: too many tensors in one call");
         a.partials = partials + used;
         LaunchScope scope(K_GRAD_NORM, bytes, stream);
-        norm_partial_kernel<kCapNorm><<<grid, kThreads, 0, stream>>>(a);
+        norm_partial_kernel<CAP><<<grid, kThreads, 0, stream>>>(a);
         MB_CUDA_CHECK(cudaGetLastError());
         used += grid;
         return OK;
@@ -1073,7 +1192,8 @@ int convert_launch(void* const* x, void* const* codes, void* const* scales, cons
       if (n > 0) {
         a.count = n;
         LaunchScope scope(K_STATE_CONVERT, elems * (sizeof(T) + 1.0 + 4.0 / kStateBlock), stream);
-        convert_kernel<T, KIND, TO_CODES, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
+        if (TO_CODES) quantize_kernel<T, KIND, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
+        else dequantize_kernel<T, KIND, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
         MB_CUDA_CHECK(cudaGetLastError());
       }
       n = 0;
@@ -1084,7 +1204,7 @@ int convert_launch(void* const* x, void* const* codes, void* const* scales, cons
     a.codes[n] = static_cast<uint8_t*>(codes[i]);
     a.scales[n] = static_cast<float*>(scales[i]);
     a.numel[n] = numel[i];
-    a.vec_ok[n] = aligned(x[i], 8 * sizeof(T)) && aligned(codes[i], 8);
+    a.vec_ok[n] = aligned(x[i], TO_CODES ? 8 * sizeof(T) : 32) && aligned(codes[i], TO_CODES ? 8 : 16);
     a.start[n + 1] = a.start[n] + (int)chunks;
     elems += (double)numel[i];
     ++n;
@@ -1096,13 +1216,16 @@ template <bool TO_CODES>
 int convert(void* const* x, void* const* codes, void* const* scales, const int64_t* numel, int count, int dtype,
             int kind, cudaStream_t stream) {
   const bool avg = kind == STATE_EXP_AVG;
-#define MB_CONVERT(T)                                                                                       \
-  return avg ? convert_launch<T, STATE_EXP_AVG, TO_CODES, kCapConvert>(x, codes, scales, numel, count, stream) \
-             : convert_launch<T, STATE_EXP_AVG_SQ, TO_CODES, kCapConvert>(x, codes, scales, numel, count, stream)
+  const bool few = count <= kCapFew;
+#define MB_CONVERT_KIND(T, KIND)                                                                    \
+  (few ? convert_launch<T, KIND, TO_CODES, kCapFew>(x, codes, scales, numel, count, stream)         \
+       : convert_launch<T, KIND, TO_CODES, kCapConvert>(x, codes, scales, numel, count, stream))
+#define MB_CONVERT(T) return avg ? MB_CONVERT_KIND(T, STATE_EXP_AVG) : MB_CONVERT_KIND(T, STATE_EXP_AVG_SQ)
   if (dtype == DT_F32) MB_CONVERT(float);
   if (dtype == DT_BF16) MB_CONVERT(__nv_bfloat16);
   MB_CONVERT(__half);
 #undef MB_CONVERT
+#undef MB_CONVERT_KIND
 }
 
 }  // namespace
@@ -1132,10 +1255,37 @@ int grad_norm_partials(int* n) {
   return rc;
 }
 
+namespace {
+template <int CAP>
+int clip_launch(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                float* out2, double* partials, cudaStream_t stream) {
+  int n = 0, launched = 0;
+  int rc = norm_partials<CAP>(tensors, numel, dtypes, count, partials, &n, stream);
+  if (rc != OK) return rc;
+  rc = for_each_norm_table<CAP>(
+      tensors, numel, dtypes, count, partials, [&](NormArgs<CAP>& a, double bytes) -> int {
+        int grid = 0;
+        const int rc = norm_grid(a.chunks, &grid);
+        if (rc != OK) return rc;
+        ++launched;
+        LaunchScope scope(K_GRAD_NORM, 2.0 * bytes, stream);
+        clip_kernel<CAP><<<grid, kThreads, 0, stream>>>(a, n, (float)max_norm, out2);
+        MB_CUDA_CHECK(cudaGetLastError());
+        return OK;
+      });
+  if (rc != OK || launched) return rc;
+  LaunchScope scope(K_GRAD_NORM, 0.0, stream);  // nothing but empty tensors: the norm is 0
+  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, 0, (float)max_norm, out2);
+  MB_CUDA_CHECK(cudaGetLastError());
+  return OK;
+}
+}  // namespace
+
 int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
                   float* out2, double* partials, cudaStream_t stream) {
   int n = 0;
-  const int rc = norm_partials(tensors, numel, dtypes, count, partials, &n, stream);
+  const int rc = count <= kCapFew ? norm_partials<kCapFew>(tensors, numel, dtypes, count, partials, &n, stream)
+                                  : norm_partials<kCapNorm>(tensors, numel, dtypes, count, partials, &n, stream);
   if (rc != OK) return rc;
   LaunchScope scope(K_GRAD_NORM, 8.0 * n, stream);
   norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, n, (float)max_norm, out2);
@@ -1145,25 +1295,8 @@ int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes,
 
 int run_clip(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
              float* out2, double* partials, cudaStream_t stream) {
-  int n = 0, launched = 0;
-  int rc = norm_partials(tensors, numel, dtypes, count, partials, &n, stream);
-  if (rc != OK) return rc;
-  rc = for_each_norm_table<kCapNorm>(
-      tensors, numel, dtypes, count, partials, [&](NormArgs<kCapNorm>& a, double bytes) -> int {
-        int grid = 0;
-        const int rc = norm_grid(a.chunks, &grid);
-        if (rc != OK) return rc;
-        ++launched;
-        LaunchScope scope(K_GRAD_NORM, 2.0 * bytes, stream);
-        clip_kernel<kCapNorm><<<grid, kThreads, 0, stream>>>(a, n, (float)max_norm, out2);
-        MB_CUDA_CHECK(cudaGetLastError());
-        return OK;
-      });
-  if (rc != OK || launched) return rc;
-  LaunchScope scope(K_GRAD_NORM, 0.0, stream);  // nothing but empty tensors: the norm is 0
-  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, 0, (float)max_norm, out2);
-  MB_CUDA_CHECK(cudaGetLastError());
-  return OK;
+  return count <= kCapFew ? clip_launch<kCapFew>(tensors, numel, dtypes, count, max_norm, out2, partials, stream)
+                          : clip_launch<kCapNorm>(tensors, numel, dtypes, count, max_norm, out2, partials, stream);
 }
 
 int run_quantize(void* const* src, void* const* codes, void* const* scales, const int64_t* numel, int count,

@@ -162,7 +162,27 @@ PyObject* collect(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"collect", collect, METH_VARARGS, "Checks tensor lists and returns their pointer tables."},
+// gradients(tensors) -> list: parameters give their .grad, other tensors themselves; None is left out.
+PyObject* gradients(PyObject*, PyObject* tensors) {
+  HANDLE_TH_ERRORS
+  Ref fast(PySequence_Fast(tensors, "a list of parameters or gradients is wanted")), out(PyList_New(0));
+  if (!fast.p || !out.p) return nullptr;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.p);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
+    int parameter = 0;  // (a plain torch.Tensor is none; a subclass may be one without being its subtype)
+    if (Py_TYPE(o) == reinterpret_cast<PyTypeObject*>(ParameterClass)) parameter = 1;
+    else if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass)) parameter = PyObject_IsInstance(o, ParameterClass);
+    if (parameter < 0) return nullptr;
+    Ref g(parameter ? PyObject_GetAttrString(o, "grad") : Py_NewRef(o));
+    if (!g.p || (g.p != Py_None && PyList_Append(out.p, g.p) < 0)) return nullptr;
+  }
+  return out.release();
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {{"gradients", gradients, METH_O, "The gradients of parameters, or the tensors themselves."},
+                         {"collect", collect, METH_VARARGS, "Checks tensor lists and returns their pointer tables."},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tables", "Pointer tables of multi-tensor calls.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

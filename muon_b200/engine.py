@@ -624,10 +624,13 @@ class CudaBackend:
             _wait_grads(torch.cuda.current_stream(device), tensors)
         out = torch.empty(2, dtype=torch.float32, device=tensors[0].device)
         need = lib.muon_b200_grad_norm_scratch_bytes()
-        # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
-        # one stream may be replayed at the same time on two.
-        scratch = (torch.empty(need + 256, dtype=torch.uint8, device=out.device)
-                   if torch.cuda.is_current_stream_capturing() else self.workspace(out.device, need, slot=5))
+        key = (device, _current_raw_stream(device), 5)
+        if torch.cuda.is_current_stream_capturing():
+            # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
+            # one stream may be replayed at the same time on two.
+            scratch = torch.empty(need + 256, dtype=torch.uint8, device=out.device)
+        elif (scratch := self._workspaces.get(key)) is None:
+            scratch = self.workspace(out.device, need, slot=5)
         _call_on(device, lib.muon_b200_clip_grads if clip else lib.muon_b200_grad_norm, tables[0], numel, codes,
                  len(tensors), max_norm, out.data_ptr(), self._aligned_ptr(scratch), need)
         self.launch_groups += 1
