@@ -6,12 +6,15 @@ importing this package fails if that library has not been built.
 """
 from ._lib import MuonB200Error, device_status  # noqa: F401  (import fails loudly without the library)
 from .adamw import (  # noqa: F401
+    AdamW,
     adamw8_step,
     adamw_step,
     clip_grad_norm_,
     dequantize_state,
+    get_adam_moments,
     grad_norm,
     quantize_state,
+    set_adam_moments,
 )
 from .backward_overlap import StepInBackward  # noqa: F401
 from .checkpoint import consolidated_state_dict, load_consolidated_state_dict  # noqa: F401
@@ -41,4 +44,5 @@ __all__ = [
     "mark_grad_ready", "StepInBackward", "consolidated_state_dict", "load_consolidated_state_dict",
     "set_ownership", "get_ownership", "ShardedMuon",
     "adamw_step", "adamw8_step", "grad_norm", "clip_grad_norm_", "quantize_state", "dequantize_state",
+    "AdamW", "set_adam_moments", "get_adam_moments",
 ]

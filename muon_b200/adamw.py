@@ -9,6 +9,7 @@ one launch takes hundreds of tensors. The formats are described in ``include/muo
 from __future__ import annotations
 
 import math
+from collections import OrderedDict
 from typing import Sequence
 
 import torch
@@ -16,7 +17,12 @@ from torch import Tensor
 
 from ._lib import STATE_BLOCK
 from ._tables import gradients
-from .engine import _STATE_KINDS, get_backend
+from .engine import _STATE_KINDS, _wait_grads, get_backend
+
+try:
+    from torch.distributed.tensor import DTensor
+except ImportError:  # pragma: no cover - torch without DTensor
+    DTensor = None
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
@@ -108,3 +114,215 @@ def dequantize_state(codes: Sequence[Tensor], scales: Sequence[Tensor], kind: st
         out = [torch.empty_like(c, dtype=dtype) for c in codes]
     get_backend().convert_state("dequantize_state", out, codes, scales, kind, False)
     return out
+
+
+# ---- moments of a parameter as optimizer state -----------------------------------------------
+# {"step", "moment_bits": 32, "exp_avg", "exp_avg_sq"} or {"step", "moment_bits": 8, "exp_avg_codes",
+# "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales"}, with "master" where master weights are kept.
+_MOMENT_KEYS = {32: ("exp_avg", "exp_avg_sq"),
+                8: ("exp_avg_codes", "exp_avg_scales", "exp_avg_sq_codes", "exp_avg_sq_scales")}
+_MIN_8BIT_NUMEL = 4096
+
+_adam_moments = "param"
+
+
+def set_adam_moments(kind: str = "param") -> None:
+    """What the auxiliary Adam of ``MuonWithAuxAdam`` and ``SingleDeviceMuonWithAuxAdam`` keeps its
+    moments in, for parameters whose state is created from now on. ``"param"`` (default): the parameter's
+    type, with the reference's arithmetic (muon.py:104-109); ``"fp32"``: float32; ``"8bit"``: 8 bits,
+    float32 for parameters of fewer than 4096 elements. The last two run ``adamw_step`` and
+    ``adamw8_step``. (Not a param-group key: the reference asserts the exact key set, muon.py:155.)"""
+    if kind not in ("param", "fp32", "8bit"):
+        raise ValueError(f"unknown kind of moments {kind!r}; expected 'param', 'fp32' or '8bit'")
+    global _adam_moments
+    _adam_moments = kind
+
+
+def get_adam_moments() -> str:
+    return _adam_moments
+
+
+def new_moments(state: dict, p: Tensor, bits: int, master: bool = False) -> None:
+    """Fill an empty ``state`` with zero moments for ``p``."""
+    state["step"] = 0
+    state["moment_bits"] = bits
+    for key in _MOMENT_KEYS[bits]:
+        if key.endswith("_scales"):
+            state[key] = torch.zeros(-(-p.numel() // STATE_BLOCK), dtype=torch.float32, device=p.device)
+        else:
+            state[key] = torch.zeros_like(p, dtype=torch.uint8 if bits == 8 else torch.float32,
+                                          memory_format=torch.preserve_format)
+    if master:
+        state["master"] = p.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
+
+
+def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
+                 grad_scale: Tensor | None = None, seed: int = 0) -> None:
+    """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out and
+    its step already counted: one call per combination of types and device."""
+    kinds: "OrderedDict[tuple, list]" = OrderedDict()
+    for p, g, state in entries:
+        if g.stride() != p.stride():  # a gradient in another order of dimensions than its parameter
+            if g.is_cuda:
+                _wait_grads(torch.cuda.current_stream(g.device), [g])
+            g = torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
+        kinds.setdefault((p.dtype, g.dtype, p.device, state["moment_bits"], "master" in state), []).append((p, g, state))
+    for (_, _, _, bits, master), members in kinds.items():
+        states = [state for _, _, state in members]
+        lists = [[state[key] for state in states] for key in _MOMENT_KEYS[bits]]
+        more = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_scale=grad_scale,
+                    masters=[state["master"] for state in states] if master else None)
+        if bits == 8:
+            more["seed"] = seed
+        (adamw8_step if bits == 8 else adamw_step)([p for p, _, _ in members], [g for _, g, _ in members], *lists,
+                                                   [state["step"] for state in states], **more)
+
+
+def convert_moments(states: Sequence[dict], bits: int) -> None:
+    """Turn the moments of these states into float32 or 8-bit ones."""
+    states = [state for state in states if state["moment_bits"] != bits]
+    by_device: dict = {}
+    for state in states:
+        by_device.setdefault(state[_MOMENT_KEYS[state["moment_bits"]][0]].device, []).append(state)
+    for members in by_device.values():
+        for kind in ("exp_avg", "exp_avg_sq"):
+            if bits == 8:
+                codes, scales = quantize_state([state[kind] for state in members], kind)
+                new = [{f"{kind}_codes": c, f"{kind}_scales": s} for c, s in zip(codes, scales)]
+            else:
+                values = dequantize_state([state[f"{kind}_codes"] for state in members],
+                                          [state[f"{kind}_scales"] for state in members], kind)
+                new = [{kind: x} for x in values]
+            for state, tensors in zip(members, new):
+                state.update(tensors)
+    for state in states:
+        for key in _MOMENT_KEYS[state["moment_bits"]]:
+            del state[key]
+        state["moment_bits"] = bits
+
+
+def restore_moments(p: Tensor, saved: dict) -> dict:
+    """The tensors of a saved state for parameter ``p``, on its device, in the types they were saved in.
+    (``torch.optim.Optimizer.load_state_dict`` casts every tensor to the parameter's type.) Moments of
+    a parameter whose dimensions lie in another order in memory than when they were saved are
+    brought into its order."""
+    keep = {k: v.detach().to(p.device, copy=True) for k, v in saved.items() if torch.is_tensor(v)}
+    laid_out = keep["exp_avg_codes" if saved["moment_bits"] == 8 else "exp_avg"]
+    if laid_out.shape != p.shape:
+        raise ValueError(f"moments of shape {tuple(laid_out.shape)} for a parameter of shape {tuple(p.shape)}")
+    if laid_out.stride() == p.stride():
+        return keep
+    state = {"moment_bits": saved["moment_bits"], **keep}
+    convert_moments([state], 32)
+    for key in ("exp_avg", "exp_avg_sq", "master"):
+        if key in state:
+            state[key] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(state[key])
+    convert_moments([state], saved["moment_bits"])
+    return {k: v for k, v in state.items() if torch.is_tensor(v)}
+
+
+class KeepsMomentTypes:
+    """``load_state_dict`` for optimizers whose state may hold ``new_moments``."""
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(ids, (p for group in self.param_groups for p in group["params"])):
+            saved = state_dict["state"].get(i, {})
+            if "moment_bits" in saved:
+                self.state[p].update(restore_moments(_local(p), saved))
+
+
+def _local(t: Tensor) -> Tensor:
+    """This rank's part of a DTensor, or the tensor itself."""
+    return t.to_local() if DTensor is not None and isinstance(t, DTensor) else t
+
+
+class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with one launch for all parameters of a type.
+
+    Arguments:
+        params, lr, betas, eps, weight_decay: as for ``torch.optim.AdamW``; parameters are float32,
+            bfloat16 or float16. Parameters without a gradient are left as they are. Of a DTensor (sharded
+            or replicated) the local part is updated and has its own moments.
+        state_bits: 32 (float32 moments whatever the parameter's type) or 8.
+        master_weights: keep a float32 copy of 16-bit parameters, which the steps are taken on.
+        min_8bit_numel: parameters with fewer elements keep float32 moments.
+        seed: of the stochastic rounding of 8-bit second moments.
+        max_grad_norm: clip the gradients of all groups together to this norm. The factor stays on the
+            device and is applied while the step reads the gradients; ``grad_norm`` holds the norm
+            of the last step. A step whose norm is not finite changes nothing (it is counted).
+
+    ``state_bits``, ``master_weights``, ``min_8bit_numel`` and ``seed`` may differ between groups. Steps are
+    counted on the host, so ``step()`` cannot be captured into a CUDA graph (``adamw_step`` can)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32,
+                 master_weights=False, min_8bit_numel=_MIN_8BIT_NUMEL, seed=0, max_grad_norm=None):
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, min_8bit_numel=min_8bit_numel, seed=seed))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        if group["state_bits"] not in (8, 32):
+            self.param_groups.pop()
+            raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW counts its steps on the host: a captured step would repeat one step number; "
+                               "capture adamw_step or adamw8_step instead")
+        work = []  # (group, [(parameter, gradient, state)])
+        sharded = False
+        for group in self.param_groups:
+            entries = []
+            for p in group["params"]:
+                g, local = p.grad, _local(p)
+                if g is None:
+                    continue
+                if local is not p:
+                    sharded = True
+                    if g.placements != p.placements:  # one that is not reduced yet, say
+                        g = g.redistribute(placements=p.placements)
+                    g = g.to_local()
+                entries.append((local, g, self.state[p]))
+            if entries:
+                work.append((group, entries))
+        if not work:
+            return loss
+        factor = None
+        if self.max_grad_norm is not None:
+            if sharded:
+                raise ValueError("max_grad_norm needs whole gradients: clip sharded ones before step() "
+                                 "(torch.nn.utils.clip_grad_norm_ takes DTensors)")
+            self.grad_norm, factor = grad_norm([g for _, entries in work for _, g, _ in entries], self.max_grad_norm)
+        for group, entries in work:
+            for local, _, state in entries:
+                if len(state) == 0:
+                    bits = 8 if group["state_bits"] == 8 and local.numel() >= group["min_8bit_numel"] else 32
+                    new_moments(state, local, bits, group["master_weights"] and local.dtype != torch.float32)
+                state["step"] += 1
+            moments_step(entries, float(group["lr"]), float(group["weight_decay"]), tuple(map(float, group["betas"])),
+                         float(group["eps"]), factor, int(group["seed"]))
+        return loss
+
+    @torch.no_grad()
+    def set_state_bits(self, bits: int) -> None:
+        """Convert the moments of all parameters, and those still to come, to 8 or 32 bits (a run that
+        goes on with another size of state, a checkpoint that was saved with one). To 8 bits: those of
+        parameters with at least ``min_8bit_numel`` elements."""
+        if bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {bits}")
+        for group in self.param_groups:
+            group["state_bits"] = bits
+            convert_moments([self.state[p] for p in group["params"] if len(self.state.get(p, {})) > 0
+                             and (bits == 32 or _local(p).numel() >= group["min_8bit_numel"])], bits)

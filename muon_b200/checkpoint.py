@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
+from .adamw import restore_moments
 from .ownership import owned_indices
 
 FORMAT = "muon_b200.consolidated.v1"
@@ -83,6 +84,10 @@ def load_consolidated_state_dict(optimizer, state) -> None:
         else:
             for i, p in enumerate(params):
                 optimizer.state.pop(p, None)
-                if i in entry.get("adam", {}):
-                    optimizer.state[p].update({k: (v.to(device=p.device, dtype=p.dtype).clone() if torch.is_tensor(v) else v)
-                                               for k, v in entry["adam"][i].items()})
+                saved = entry.get("adam", {}).get(i)
+                if saved is None:
+                    continue
+                optimizer.state[p].update({k: (v.to(device=p.device, dtype=p.dtype).clone() if torch.is_tensor(v) else v)
+                                           for k, v in saved.items()})
+                if "moment_bits" in saved:  # moments in float32 or 8 bits keep their types (adamw.py)
+                    optimizer.state[p].update(restore_moments(p, saved))

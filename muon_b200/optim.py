@@ -18,6 +18,7 @@ from collections import OrderedDict
 import torch
 import torch.distributed as dist
 
+from .adamw import _MIN_8BIT_NUMEL, KeepsMomentTypes, get_adam_moments, moments_step, new_moments
 from .engine import get_backend, plan_launches, view_2d
 from .exchange import get_peer_push
 from .ownership import get_ownership, owners
@@ -72,13 +73,22 @@ def _adam_update_params(optimizer, group) -> None:
             p.grad = p.grad.contiguous()
         state = optimizer.state[p]
         if len(state) == 0:
-            state["exp_avg"] = torch.zeros_like(p)
-            state["exp_avg_sq"] = torch.zeros_like(p)
-            state["step"] = 0
+            moments = get_adam_moments()
+            if moments == "param":
+                state["exp_avg"] = torch.zeros_like(p)
+                state["exp_avg_sq"] = torch.zeros_like(p)
+                state["step"] = 0
+            else:
+                new_moments(state, p, 8 if moments == "8bit" and p.numel() >= _MIN_8BIT_NUMEL else 32)
         state["step"] += 1
+    own = [p for p in params if "moment_bits" in optimizer.state[p]]  # moments in float32 or 8 bits
+    if own:
+        moments_step([(p, p.grad, optimizer.state[p]) for p in own], group["lr"], group["weight_decay"],
+                     group["betas"], group["eps"])
     by_kind: "OrderedDict[tuple, list]" = OrderedDict()
     for p in params:
-        by_kind.setdefault((p.dtype, p.device), []).append(p)
+        if "moment_bits" not in optimizer.state[p]:
+            by_kind.setdefault((p.dtype, p.device), []).append(p)
     for plist in by_kind.values():
         backend.adam_step(plist, [p.grad for p in plist],
                           [optimizer.state[p]["exp_avg"] for p in plist],
@@ -255,7 +265,7 @@ def _apply_group_defaults(param_groups, sort_muon_params: bool) -> None:
             assert set(group.keys()) == set(["params", "lr", "betas", "eps", "weight_decay", "use_muon"])
 
 
-class MuonWithAuxAdam(torch.optim.Optimizer):
+class MuonWithAuxAdam(KeepsMomentTypes, torch.optim.Optimizer):
     """Distributed Muon with an internal Adam for the parameters Muon does not suit
     (muon.py:112-199). Every group carries ``use_muon``; Muon groups accept ``lr``,
     ``momentum``, ``weight_decay``; Adam groups accept ``lr``, ``betas``, ``eps``,
@@ -279,7 +289,7 @@ class MuonWithAuxAdam(torch.optim.Optimizer):
         return loss
 
 
-class SingleDeviceMuonWithAuxAdam(torch.optim.Optimizer):
+class SingleDeviceMuonWithAuxAdam(KeepsMomentTypes, torch.optim.Optimizer):
     """Non-distributed variant of MuonWithAuxAdam (muon.py:202-260)."""
 
     def __init__(self, param_groups):

@@ -122,3 +122,234 @@ def test_pointer_tables_refuse_what_is_no_cuda_tensor():
         collect("grad_norm", (("gradient", 5, 7, 0, False),))
     device, numel, tables, found, codes = collect("grad_norm", (("gradient", [], 7, 0, False),))
     assert (device, numel, tables, found, codes) == (-1, b"", (b"",), (0,), b"")
+
+
+# ------------------------------------------------------------------------------- the classes, without a GPU
+class _OracleBackend:
+    """Stand-in for the CUDA backend: the same calls on CPU tensors, from the oracle."""
+
+    def __init__(self):
+        self.calls = []
+
+    def adamw_step(self, params, grads, ms, vs, steps, lr, weight_decay, betas, eps, masters, grad_scale):
+        self.calls.append(("adamw", len(params), params[0].dtype, masters is not None))
+        f = 1.0 if grad_scale is None else float(grad_scale)
+        for i, p in enumerate(params):
+            w = p if masters is None else masters[i]
+            new = orc.adamw64(w, grads[i], ms[i], vs[i], steps[i], lr, betas, eps, weight_decay, f)
+            w.copy_(new[0])
+            p.copy_(w)
+            ms[i].copy_(new[1])
+            vs[i].copy_(new[2])
+
+    def adamw8_step(self, params, grads, mc, msc, vc, vsc, steps, lr, weight_decay, betas, eps, masters, grad_scale, seed):
+        self.calls.append(("adamw8", len(params), params[0].dtype, masters is not None))
+        f = 1.0 if grad_scale is None else float(grad_scale)
+        for i, p in enumerate(params):
+            m = orc.dequantize(mc[i], msc[i], "exp_avg").view_as(p)
+            v = orc.dequantize(vc[i], vsc[i], "exp_avg_sq").view_as(p)
+            w = p if masters is None else masters[i]
+            w.copy_(orc.adamw64(w, grads[i], m, v, steps[i], lr, betas, eps, weight_decay, f)[0])
+            p.copy_(w)
+            m, v = orc.moments32(grads[i], m, v, betas, f)
+            for x, c, s, kind, bits in ((m, mc[i], msc[i], "exp_avg", None),
+                                        (v, vc[i], vsc[i], "exp_avg_sq", orc.random_bits(p.numel(), seed, steps[i]))):
+                codes, scales = orc.quantize(x.reshape(-1), kind, bits)
+                c.view(-1).copy_(codes)
+                s.copy_(scales)
+
+    def grad_norm(self, tensors, max_norm, clip):
+        norm = math.sqrt(sum(float(t.double().square().sum()) for t in tensors))
+        return torch.tensor([norm, min(1.0, max_norm / (norm + 1e-6))])
+
+    def convert_state(self, what, values, codes, scales, kind, to_codes):
+        for x, c, s in zip(values, codes, scales):
+            if to_codes:
+                new_c, new_s = orc.quantize(x.reshape(-1), kind)
+                c.view(-1).copy_(new_c)
+                s.copy_(new_s)
+            else:
+                x.view(-1).copy_(orc.dequantize(c, s, kind))
+
+    def adam_step(self, params, grads, ms, vs, steps, lr, weight_decay, betas, eps):
+        self.calls.append(("adam", len(params), params[0].dtype, False))
+
+
+@pytest.fixture
+def backend():
+    from muon_b200 import engine
+    stand_in = _OracleBackend()
+    prev = engine._set_backend_for_testing(stand_in)
+    yield stand_in
+    engine._set_backend_for_testing(prev)
+
+
+def _params(seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    shapes = [(64, 80), (5,), (70, 3, 5, 5), (4096,)]
+    kinds = [torch.float32, torch.float32, torch.bfloat16, torch.bfloat16]
+    return [torch.nn.Parameter((torch.randn(s, generator=gen) * 0.1).to(k)) for s, k in zip(shapes, kinds)]
+
+
+def _give_grads(params, seed):
+    gen = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.shape, generator=gen) * 0.01).to(p.dtype)
+
+
+def test_adamw_class_groups_and_state(backend):
+    import muon_b200 as mb
+    params = _params()
+    opt = mb.AdamW([dict(params=params[:2], lr=1e-2), dict(params=params[2:], state_bits=8, master_weights=True)],
+                   weight_decay=0.0)
+    opt.step()
+    assert backend.calls == [] and len(opt.state) == 0  # nothing has a gradient
+    _give_grads(params, 1)
+    params[1].grad = None
+    before = params[1].detach().clone()
+    opt.step()
+    assert backend.calls == [("adamw", 1, torch.float32, False), ("adamw8", 2, torch.bfloat16, True)]
+    assert torch.equal(params[1], before) and len(opt.state.get(params[1], {})) == 0
+    assert set(opt.state[params[0]]) == {"step", "moment_bits", "exp_avg", "exp_avg_sq"}
+    s = opt.state[params[2]]
+    assert s["exp_avg_codes"].dtype == torch.uint8 and s["exp_avg_codes"].shape == params[2].shape
+    assert s["exp_avg_scales"].shape == (21,) and s["master"].dtype == torch.float32
+    want = torch.optim.AdamW([params[0].detach().clone().requires_grad_()], lr=1e-2)  # the first step is lr * sign
+    assert (opt.state[params[0]]["step"], s["step"]) == (1, 1) and want is not None
+    backend.calls.clear()
+    opt = mb.AdamW(params, state_bits=8, min_8bit_numel=4096 + 1)
+    _give_grads(params, 2)
+    opt.step()
+    # by type and by size of state, in the order they come
+    assert backend.calls == [("adamw8", 1, torch.float32, False), ("adamw", 1, torch.float32, False),
+                             ("adamw8", 1, torch.bfloat16, False), ("adamw", 1, torch.bfloat16, False)]
+
+
+def test_adamw_class_agrees_with_torch(backend):
+    """Two steps on float32 parameters: the stand-in computes in 64 bits, torch in 32 (a few roundings)."""
+    import muon_b200 as mb
+    gen = torch.Generator().manual_seed(3)
+    a = torch.nn.Parameter(torch.randn(50, 7, generator=gen))
+    b = torch.nn.Parameter(a.detach().clone())
+    ours, theirs = mb.AdamW([a], lr=1e-2, weight_decay=0.1), torch.optim.AdamW([b], lr=1e-2, weight_decay=0.1)
+    for k in range(2):
+        a.grad = torch.randn(50, 7, generator=gen)
+        b.grad = a.grad.clone()
+        ours.step()
+        theirs.step()
+        assert torch.allclose(a, b, rtol=1e-6, atol=1e-7)
+
+
+def test_adamw_class_clips_all_groups_together(backend):
+    import muon_b200 as mb
+    gen = torch.Generator().manual_seed(4)
+    ps = [torch.nn.Parameter(torch.randn(40, generator=gen)) for _ in range(3)]
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    opt = mb.AdamW([dict(params=ps[:1]), dict(params=ps[1:])], max_grad_norm=0.5)
+    ref = mb.AdamW([dict(params=qs[:1]), dict(params=qs[1:])])
+    for p, q in zip(ps, qs):
+        p.grad = torch.randn(40, generator=gen)
+        q.grad = p.grad.clone()
+    torch.nn.utils.clip_grad_norm_(qs, 0.5)
+    opt.step()
+    ref.step()
+    assert float(opt.grad_norm) == pytest.approx(float(torch.cat([p.grad for p in ps]).norm()), rel=1e-6)
+    for p, q in zip(ps, qs):
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-7)
+        assert torch.allclose(opt.state[p]["exp_avg"], ref.state[q]["exp_avg"], rtol=1e-5, atol=1e-9)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_class_state_dict_keeps_types(backend, bits, tmp_path):
+    import muon_b200 as mb
+    params = _params(5)
+    opt = mb.AdamW(params, state_bits=bits, master_weights=True)
+    for k in range(2):
+        _give_grads(params, 10 + k)
+        opt.step()
+    torch.save(opt.state_dict(), tmp_path / "state.pt")
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = mb.AdamW(copies, state_bits=40 - bits)
+    again.load_state_dict(torch.load(tmp_path / "state.pt"))
+    for p, q in zip(params, copies):
+        a, b = opt.state[p], again.state[q]
+        assert set(a) == set(b)
+        for k in a:
+            assert type(a[k]) is type(b[k])
+            if torch.is_tensor(a[k]):
+                assert a[k].dtype == b[k].dtype and torch.equal(a[k], b[k]) and a[k].data_ptr() != b[k].data_ptr(), k
+            else:
+                assert a[k] == b[k]
+    _give_grads(params, 12)
+    _give_grads(copies, 12)
+    opt.step()
+    again.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, copies))
+    bad = opt.state_dict()
+    bad["state"][0]["exp_avg" if bits == 32 else "exp_avg_codes"] = torch.zeros(3)
+    with pytest.raises(ValueError, match="moments of shape"):
+        again.load_state_dict(bad)
+
+
+def test_adamw_class_changes_its_state_bits(backend):
+    import muon_b200 as mb
+    params = _params(6)
+    opt = mb.AdamW(params)
+    _give_grads(params, 1)
+    opt.step()
+    m = opt.state[params[0]]["exp_avg"].clone()
+    opt.set_state_bits(8)
+    assert [opt.state[p]["moment_bits"] for p in params] == [8, 32, 8, 8]
+    assert opt.param_groups[0]["state_bits"] == 8 and "exp_avg" not in opt.state[params[0]]
+    _give_grads(params, 2)
+    opt.step()
+    opt.set_state_bits(32)
+    assert all(opt.state[p]["moment_bits"] == 32 and opt.state[p]["exp_avg"].shape == p.shape for p in params)
+    assert [opt.state[p]["step"] for p in params] == [2] * 4 and m.shape == params[0].shape
+    for bad in (16, "8"):
+        with pytest.raises(ValueError, match="state_bits"):
+            opt.set_state_bits(bad)
+        with pytest.raises(ValueError, match="state_bits"):
+            mb.AdamW(_params(), state_bits=bad)
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        mb.AdamW(_params(), max_grad_norm=-1.0)
+
+
+def test_auxiliary_adam_keeps_other_moments_when_asked(backend):
+    """set_adam_moments: state made from then on; what exists keeps its kind; the default is the
+    reference's arithmetic on the parameter's type."""
+    import copy
+    import muon_b200 as mb
+    params = _params(7)
+    assert mb.get_adam_moments() == "param"
+    opt = mb.SingleDeviceMuonWithAuxAdam([dict(params=params[:1], use_muon=False)])
+    _give_grads(params, 1)
+    opt.step()
+    assert backend.calls == [("adam", 1, torch.float32, False)] and "moment_bits" not in opt.state[params[0]]
+    try:
+        mb.set_adam_moments("8bit")
+        opt.step()
+        aux = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)])
+        params[1].grad = None  # the reference's rule: zeros
+        aux.step()
+        mb.set_adam_moments("fp32")
+        wide = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)])
+        wide.step()
+        with pytest.raises(ValueError, match="moments"):
+            mb.set_adam_moments("int8")
+    finally:
+        mb.set_adam_moments()
+    assert backend.calls[1][0] == "adam"
+    assert [aux.state[p]["moment_bits"] for p in params] == [8, 32, 8, 8]
+    assert [wide.state[p]["moment_bits"] for p in params] == [32] * 4
+    assert wide.state[params[2]]["exp_avg"].dtype == torch.float32 and (params[1].grad == 0).all()
+    for source in (aux, wide):
+        target = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)])
+        target.load_state_dict(copy.deepcopy(source.state_dict()))
+        other = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)])
+        mb.load_consolidated_state_dict(other, mb.consolidated_state_dict(source))
+        for p in params:
+            for key, value in source.state[p].items():
+                for to in (target, other):
+                    got = to.state[p][key]
+                    assert (got.dtype == value.dtype and torch.equal(got, value)) if torch.is_tensor(value) else got == value
