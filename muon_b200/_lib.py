@@ -105,7 +105,7 @@ PROTOTYPES = {
     "muon_b200_adam": (c_int, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p),
                                POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64), c_int, c_int,
                                c_double, c_double, c_double, c_double, c_double, c_void_p]),
-    # (tables of the calls below are passed as addresses, see address_table)
+    # (the package makes these calls through _tables; tables are addresses here)
     "muon_b200_adamw": (c_int, [c_void_p] * 7 + [c_int, c_int, c_int] + [c_double] * 5 + [c_void_p, c_void_p]),
     "muon_b200_adamw8": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int] + [c_double] * 5
                          + [c_uint32, c_void_p, c_void_p]),
@@ -144,12 +144,6 @@ def ptr_array(ptrs) -> ctypes.Array:
 
 def i64_array(vals) -> ctypes.Array:
     return (c_int64 * len(vals))(*vals)
-
-
-def address(table) -> int:
-    """Address of an ``array.array`` (a table of pointers, sizes or steps). The caller keeps the array
-    alive until the call has returned."""
-    return table.buffer_info()[0]
 
 
 def device_status(reset: bool = True) -> int:

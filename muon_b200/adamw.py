@@ -75,7 +75,7 @@ def grad_norm(tensors, max_norm: float = math.inf) -> tuple[Tensor, Tensor]:
     tensors = _gradients(tensors)
     if not tensors:
         return torch.zeros(()), torch.ones(())
-    return get_backend().grad_norm(tensors, max_norm, clip=False).unbind()
+    return get_backend().grad_norm(tensors, max_norm, clip=False)
 
 
 def clip_grad_norm_(tensors, max_norm: float) -> Tensor:

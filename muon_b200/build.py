@@ -1,5 +1,5 @@
-"""Builds ``libmuon_b200.so`` (the C-ABI CUDA library) and ``_tables.so`` (the Python extension that
-lays out pointer tables) in-tree, with nvcc for sm_100a and the host compiler.
+"""Builds ``libmuon_b200.so`` (the C-ABI CUDA library) and ``_tables.so`` (the Python extension that makes
+its multi-tensor calls from lists of tensors) in-tree, with nvcc for sm_100a and the host compiler.
 
 Usage: ``python muon_b200/build.py [--force] [-v]``. Run it as a script: importing the
 package needs the library to exist already. nvcc cross-compiles, so no GPU is needed.
@@ -21,7 +21,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libmuon_b200.so")
 TABLES_PATH = os.path.join(PKG_DIR, "_tables.so")
 SOURCES = ("api.cu", "ns_driver.cu", "ns_gemm.cu", "elementwise.cu", "adamw.cu", "profiling.cu", "peer.cu", "no_alloc.cu")
 HEADERS = ("common.cuh", "ns_driver.h", "ns_gemm.h", "elementwise.h", "adamw.h", "profiling.h", os.path.join("..", "..", "include", "muon_b200.h"))
-TABLES_SOURCE = "tables.cpp"
+TABLES_SOURCES = ("tables.cpp", os.path.join("..", "..", "include", "muon_b200.h"))
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
@@ -45,7 +45,7 @@ def _older(target: str, names) -> bool:
 
 
 def is_stale() -> bool:
-    return _older(LIB_PATH, SOURCES + HEADERS) or _older(TABLES_PATH, (TABLES_SOURCE,))
+    return _older(LIB_PATH, SOURCES + HEADERS) or _older(TABLES_PATH, TABLES_SOURCES)
 
 
 def _run(cmd, verbose: bool = False) -> None:
@@ -67,18 +67,20 @@ def _build_tables(verbose: bool) -> None:
     compiler = shutil.which("g++") or shutil.which("c++")
     if compiler is None:
         raise RuntimeError("no C++ compiler found: cannot build _tables.so")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    # (torch's libraries are loaded already when the extension is; libmuon_b200.so lies beside it)
     _run([compiler, "-O2", "-std=c++17", "-shared", "-fPIC", "-I" + include,
           "-I" + os.path.join(include, "torch", "csrc", "api", "include"),
-          "-I" + sysconfig.get_paths()["include"], "-o", TABLES_PATH, os.path.join(CSRC, TABLES_SOURCE),
-          "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"], verbose)
+          "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"),
+          "-o", TABLES_PATH, os.path.join(CSRC, TABLES_SOURCES[0]),
+          "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+          "-L" + PKG_DIR, "-lmuon_b200", "-Wl,-rpath,$ORIGIN"], verbose)
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile what is missing or older than its sources, files side by side. Returns the library's path."""
     jobs = []
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor() as pool:
-        if force or _older(TABLES_PATH, (TABLES_SOURCE,)):
-            jobs.append(pool.submit(_build_tables, verbose))
         objects = []
         if force or _older(LIB_PATH, SOURCES + HEADERS):
             for name in SOURCES:
@@ -90,6 +92,8 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             job.result()
         if objects:
             _run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects], verbose)
+    if force or _older(TABLES_PATH, TABLES_SOURCES):
+        _build_tables(verbose)
     return LIB_PATH
 
 

@@ -965,6 +965,9 @@ struct ListStart {
 // The first element, under N, at which all lists are aligned to N elements; kNoHead: there is none.
 template <int N>
 int common_head(std::initializer_list<ListStart> lists) {
+  uintptr_t off = 0;  // (a null pointer is aligned)
+  for (const ListStart& l : lists) off |= reinterpret_cast<uintptr_t>(l.p) & (N * l.bytes - 1);
+  if (off == 0) return 0;
   int head = -1;
   for (const ListStart& l : lists) {
     if (!l.p) continue;
@@ -973,7 +976,7 @@ int common_head(std::initializer_list<ListStart> lists) {
     if (head >= 0 && h != head) return kNoHead;
     head = h;
   }
-  return head < 0 ? 0 : head;
+  return head;
 }
 
 // Adds `chunks` to the running total of a launch; false when the launch must go out first.
@@ -1043,7 +1046,8 @@ int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t st
   BiasCorrection bias;
   const double bytes = (MASTER ? sizeof(P) + 8.0 : 2.0 * sizeof(P)) + sizeof(G) + 4.0 + 16.0 / kStateBlock;
   constexpr int kShared = kShared8<P, G, MASTER>;
-  MB_CUDA_CHECK(cudaFuncSetAttribute(adamw8_kernel<P, G, MASTER, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
+  if (kShared > 48 * 1024)
+    MB_CUDA_CHECK(cudaFuncSetAttribute(adamw8_kernel<P, G, MASTER, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared));
   int sms = 0, rc = device_sm_count(&sms);
   if (rc != OK) return rc;
   double blocks = 0;

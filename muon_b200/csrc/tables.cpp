@@ -1,10 +1,15 @@
-// Python extension `muon_b200._tables`: checks the tensor lists of a multi-tensor call and lays out
-// their pointer tables. With hundreds of tensors and five lists, the same checks written in Python take
-// longer than the kernel of the call. No arithmetic and no CUDA call happens here; the tables go to the
-// C entry points of libmuon_b200.
+// Python extension `muon_b200._tables`: multi-tensor calls from lists of tensors. It checks the lists, lays
+// out their pointer tables and calls the C entry points of libmuon_b200 (include/muon_b200.h) on the current
+// stream of the tensors' device. With hundreds of tensors and five lists the same checks written in
+// Python take longer than the kernel of the call. No arithmetic happens here.
 #include <Python.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "../../include/muon_b200.h"
 
 #include <algorithm>
 #include <cstdint>
@@ -13,29 +18,20 @@
 
 namespace {
 
-constexpr int kStateBlock = 256;  // elements per scale of 8-bit state (MUON_B200_STATE_BLOCK)
-
 // Bits of the element types, in the order of the MUON_B200_F32, _BF16, _F16 codes; then uint8.
+constexpr int kF32 = 1, kBF16 = 2, kF16 = 4, kU8 = 8, kFloats = 7;
 int type_bit(at::ScalarType t) {
   switch (t) {
-    case at::kFloat: return 1;
-    case at::kBFloat16: return 2;
-    case at::kHalf: return 4;
-    case at::kByte: return 8;
+    case at::kFloat: return kF32;
+    case at::kBFloat16: return kBF16;
+    case at::kHalf: return kF16;
+    case at::kByte: return kU8;
     default: return 0;
   }
 }
+int type_code(int bit) { return bit == kF32 ? MUON_B200_F32 : bit == kBF16 ? MUON_B200_BF16 : MUON_B200_F16; }
 const char* type_names(int mask) {
-  switch (mask) {
-    case 1: return "float32";
-    case 8: return "uint8";
-    case 7: return "float32, bfloat16 or float16";
-    case 3: return "float32 or bfloat16";
-    case 5: return "float32 or float16";
-    case 2: return "bfloat16";
-    case 4: return "float16";
-    default: return "of a supported type";
-  }
+  return mask == kF32 ? "float32" : mask == kU8 ? "uint8" : "float32, bfloat16 or float16";
 }
 
 struct Ref {  // owned reference
@@ -48,124 +44,269 @@ struct Ref {  // owned reference
 };
 
 using Range = std::pair<uintptr_t, uintptr_t>;
+using Table = std::vector<void*>;
+enum Layout { kLikeFirst, kScales };  // sizes of a list: those of the first list, or one per block of its elements
 
-// Sorted `more` into sorted `all`; false when two ranges overlap. Lists mostly come in ascending order of
-// address, so this is linear.
-bool merge_ranges(std::vector<Range>& all, std::vector<Range>& more) {
-  if (!std::is_sorted(more.begin(), more.end())) std::sort(more.begin(), more.end());
-  const size_t middle = all.size();
-  all.insert(all.end(), more.begin(), more.end());
-  std::inplace_merge(all.begin(), all.begin() + middle, all.end());
-  for (size_t i = 1; i < all.size(); ++i)
-    if (all[i - 1].second > all[i].first) return false;
-  return true;
-}
-
-// collect(what, ((name, tensors, types, layout, written), ...)) ->
-//   (device index, numel table, (address table per list, ...), (types found per list, ...), type codes of list 0)
-// types: mask of type_bit; layout 0: the sizes and strides of the first list, 1: one float per
-// kStateBlock elements of it; written: must not overlap another written tensor.
-PyObject* collect(PyObject*, PyObject* args) {
-  HANDLE_TH_ERRORS
+// The lists of one call. All tensors are on one device; what is written does not overlap.
+struct Lists {
   const char* what;
-  PyObject* lists;
-  if (!PyArg_ParseTuple(args, "sO!", &what, &PyTuple_Type, &lists)) return nullptr;
-  const Py_ssize_t n_lists = PyTuple_GET_SIZE(lists);
-  Ref tables(PyTuple_New(n_lists)), found(PyTuple_New(n_lists)), numel_table, code_table, first_fast;
-  if (!tables.p || !found.p) return nullptr;
   Py_ssize_t n = 0;
   int64_t device = -1;
-  int64_t* numel = nullptr;
-  int32_t* codes = nullptr;
-  std::vector<Range> written_ranges, ranges;
-  for (Py_ssize_t l = 0; l < n_lists; ++l) {
-    const char* name;
-    PyObject* tensors;
-    int types, layout, written;
-    if (!PyArg_ParseTuple(PyTuple_GET_ITEM(lists, l), "sOiip", &name, &tensors, &types, &layout, &written)) return nullptr;
+  std::vector<int64_t> numel;
+  std::vector<int> codes;  // element types of the first list
+  std::vector<Range> written;
+  Ref first;
+
+  explicit Lists(const char* w) : what(w) {}
+
+  // Adds a list; false with a Python error set. `found`: mask of the types in it.
+  bool add(const char* name, PyObject* tensors, int types, Layout layout, bool writes, Table& table, int& found) {
     Ref fast(PySequence_Fast(tensors, "lists of tensors are lists or tuples"));
-    if (!fast.p) return nullptr;
+    if (!fast.p) return false;
     const Py_ssize_t count = PySequence_Fast_GET_SIZE(fast.p);
-    if (l == 0) {
+    const bool is_first = first.p == nullptr;
+    if (is_first) {
       n = count;
-      numel_table.p = PyBytes_FromStringAndSize(nullptr, n * 8);
-      code_table.p = PyBytes_FromStringAndSize(nullptr, n * 4);
-      if (!numel_table.p || !code_table.p) return nullptr;
-      numel = reinterpret_cast<int64_t*>(PyBytes_AS_STRING(numel_table.p));
-      codes = reinterpret_cast<int32_t*>(PyBytes_AS_STRING(code_table.p));
+      numel.resize(n);
+      codes.resize(n);
     } else if (count != n) {
-      return PyErr_Format(PyExc_ValueError, "%s: %zd %s tensors for %zd tensors", what, count, name, n);
+      PyErr_Format(PyExc_ValueError, "%s: %zd %s tensors for %zd tensors", what, count, name, n);
+      return false;
     }
-    Ref table(PyBytes_FromStringAndSize(nullptr, n * 8));
-    if (!table.p) return nullptr;
-    uint64_t* address = reinterpret_cast<uint64_t*>(PyBytes_AS_STRING(table.p));
-    int mask = 0;
-    ranges.clear();
+    table.resize(n);
+    found = 0;
+    std::vector<Range> ranges;
+    if (writes) ranges.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
-      if (!THPVariable_Check(o))
-        return PyErr_Format(PyExc_TypeError, "%s: %s %zd is no tensor but %.80s", what, name, i, Py_TYPE(o)->tp_name);
+      if (!THPVariable_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "%s: %s %zd is no tensor but %.80s", what, name, i, Py_TYPE(o)->tp_name);
+        return false;
+      }
       const at::Tensor& t = THPVariable_Unpack(o);
-      if (!t.is_cuda())
-        return PyErr_Format(PyExc_RuntimeError,
-                            "muon_b200: every %s tensor of %s must live on a CUDA (sm_100) device, got device=%s; "
-                            "there is no CPU implementation",
-                            name, what, t.device().str().c_str());
+      if (!t.is_cuda()) {
+        PyErr_Format(PyExc_RuntimeError,
+                     "muon_b200: every %s tensor of %s must live on a CUDA (sm_100) device, got device=%s; "
+                     "there is no CPU implementation", name, what, t.device().str().c_str());
+        return false;
+      }
       if (device < 0) device = t.get_device();
-      else if (t.get_device() != device)
-        return PyErr_Format(PyExc_ValueError, "%s: %s tensors must all be on cuda:%lld, got %s", what, name,
-                            (long long)device, t.device().str().c_str());
+      if (t.get_device() != device) {
+        PyErr_Format(PyExc_ValueError, "%s: %s tensors must all be on cuda:%lld, got %s", what, name,
+                     (long long)device, t.device().str().c_str());
+        return false;
+      }
       const int bit = type_bit(t.scalar_type());
       if (!(bit & types)) {
         Ref dtype(PyObject_GetAttrString(o, "dtype"));
-        if (!dtype.p) return nullptr;
-        return PyErr_Format(PyExc_ValueError, "%s: %s tensors must be %s, got %S", what, name, type_names(types), dtype.p);
+        if (dtype.p)
+          PyErr_Format(PyExc_ValueError, "%s: %s tensors must be %s, got %S", what, name, type_names(types), dtype.p);
+        return false;
       }
-      mask |= bit;
-      if (!t.has_storage())
-        return PyErr_Format(PyExc_ValueError, "%s: %s %zd has no memory of its own (a sharded tensor? pass its local part)",
-                            what, name, i);
+      found |= bit;
+      if (!t.has_storage()) {
+        PyErr_Format(PyExc_ValueError, "%s: %s %zd has no memory of its own", what, name, i);
+        return false;
+      }
       const int64_t size = t.numel();
       bool dense;
-      if (l == 0) {
+      if (is_first) {
         numel[i] = size;
-        codes[i] = bit == 1 ? 0 : bit == 2 ? 1 : 2;
+        codes[i] = type_code(bit);
         dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
       } else {
-        const at::Tensor& ref = THPVariable_Unpack(PySequence_Fast_GET_ITEM(first_fast.p, i));
-        const int64_t want = layout == 0 ? numel[i] : (numel[i] + kStateBlock - 1) / kStateBlock;
-        if (size != want)
-          return PyErr_Format(PyExc_ValueError, "%s: %s tensor %zd has another number of elements than it must have "
-                              "(%lld, not %lld)", what, name, i, (long long)size, (long long)want);
-        dense = t.is_contiguous() && (layout == 1 || ref.is_contiguous());
-        if (!dense && layout == 0)
-          dense = t.sizes() == ref.sizes() && t.strides() == ref.strides();  // ref is dense
+        const at::Tensor& ref = THPVariable_Unpack(PySequence_Fast_GET_ITEM(first.p, i));
+        const int64_t want =
+            layout == kLikeFirst ? numel[i] : (numel[i] + MUON_B200_STATE_BLOCK - 1) / MUON_B200_STATE_BLOCK;
+        if (size != want) {
+          PyErr_Format(PyExc_ValueError, "%s: %s tensor %zd has another number of elements than it must have "
+                       "(%lld, not %lld)", what, name, i, (long long)size, (long long)want);
+          return false;
+        }
+        dense = t.is_contiguous() && (layout == kScales || ref.is_contiguous());
+        if (!dense && layout == kLikeFirst)  // the first list's tensor is dense
+          dense = t.sizes() == ref.sizes() && t.strides() == ref.strides();
       }
-      if (!dense && size > 1)
-        return PyErr_Format(PyExc_ValueError, "%s: %s tensors must be contiguous, or dense with the strides of the "
-                            "tensor they belong to (tensor %zd)", what, name, i);
-      void* p = size == 0 ? nullptr : written ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
-      address[i] = reinterpret_cast<uint64_t>(p);
-      if (written && size > 0)
-        ranges.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + size * t.element_size());
+      if (!dense && size > 1) {
+        PyErr_Format(PyExc_ValueError, "%s: %s tensors must be contiguous, or dense with the strides of the tensor they "
+                     "belong to (tensor %zd)", what, name, i);
+        return false;
+      }
+      table[i] = size == 0 ? nullptr : writes ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
+      if (writes && size > 0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(table[i]);
+        ranges.emplace_back(at, at + size * t.element_size());
+      }
     }
-    if (written && !merge_ranges(written_ranges, ranges))
-      return PyErr_Format(PyExc_ValueError, "%s: memory that is written (%s) appears twice in the call", what, name);
-    PyObject* m = PyLong_FromLong(mask);
-    if (!m) return nullptr;
-    PyTuple_SET_ITEM(found.p, l, m);
-    PyTuple_SET_ITEM(tables.p, l, table.release());
-    if (l == 0) first_fast.p = fast.release();
+    if (is_first) first.p = fast.release();
+    if (writes && !merge(ranges)) {
+      PyErr_Format(PyExc_ValueError, "%s: memory that is written (%s) appears twice in the call", what, name);
+      return false;
+    }
+    return true;
   }
-  return Py_BuildValue("LNNNN", (long long)device, numel_table.release(), tables.release(), found.release(),
-                       code_table.release());
+
+  // Sorted `more` into the sorted written ranges; false when two overlap. Lists mostly come in ascending
+  // order of address, so this is linear.
+  bool merge(std::vector<Range>& more) {
+    if (!std::is_sorted(more.begin(), more.end())) std::sort(more.begin(), more.end());
+    const size_t middle = written.size();
+    written.insert(written.end(), more.begin(), more.end());
+    std::inplace_merge(written.begin(), written.begin() + middle, written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i - 1].second > written[i].first) return false;
+    return true;
+  }
+
+  // The code of a list that must have one type; -1 with a Python error set.
+  int one_type(int mask, const char* name) const {
+    if (!(mask & (mask - 1))) return type_code(mask);
+    PyErr_Format(PyExc_ValueError, "%s needs %s tensors of one dtype", what, name);
+    return -1;
+  }
+};
+
+// steps: one integer for all, or a sequence of n.
+bool read_steps(const Lists& lists, PyObject* o, std::vector<int64_t>& steps) {
+  steps.resize(lists.n);
+  if (PyLong_Check(o)) {
+    const int64_t s = PyLong_AsLongLong(o);
+    if (s == -1 && PyErr_Occurred()) return false;
+    std::fill(steps.begin(), steps.end(), s);
+    return true;
+  }
+  Ref fast(PySequence_Fast(o, "steps are an integer or a list of integers"));
+  if (!fast.p) return false;
+  if (PySequence_Fast_GET_SIZE(fast.p) != lists.n) {
+    PyErr_Format(PyExc_ValueError, "%s: %zd steps for %zd tensors", lists.what, PySequence_Fast_GET_SIZE(fast.p), lists.n);
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < lists.n; ++i) {
+    steps[i] = PyLong_AsLongLong(PySequence_Fast_GET_ITEM(fast.p, i));
+    if (steps[i] == -1 && PyErr_Occurred()) return false;
+  }
+  return true;
+}
+
+// adamw(params, grads, masters or None, (moment lists), steps, lr, weight_decay, beta1, beta2, eps,
+//       grad_scale or None, seed) -> status. Two moment lists: float32; four: 8-bit codes and scales of both.
+PyObject* adamw(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *params, *grads, *masters, *moments, *steps_o, *scale;
+  double lr, wd, b1, b2, eps;
+  unsigned int seed;
+  if (!PyArg_ParseTuple(args, "OOOO!OdddddOI", &params, &grads, &masters, &PyTuple_Type, &moments, &steps_o, &lr, &wd,
+                        &b1, &b2, &eps, &scale, &seed))
+    return nullptr;
+  const bool eight = PyTuple_GET_SIZE(moments) == 4;
+  if (!eight && PyTuple_GET_SIZE(moments) != 2) return PyErr_Format(PyExc_ValueError, "two or four lists of moments");
+  Lists lists(eight ? "adamw8_step" : "adamw_step");
+  Table p, g, w, m[4];
+  int p_types = 0, g_types = 0, found = 0;
+  const bool has_masters = masters != Py_None;
+  if (!lists.add("parameter", params, kFloats, kLikeFirst, true, p, p_types) ||
+      !lists.add("gradient", grads, kFloats, kLikeFirst, false, g, g_types) ||
+      (has_masters && !lists.add("master", masters, kF32, kLikeFirst, true, w, found)))
+    return nullptr;
+  static const char* const names32[] = {"exp_avg", "exp_avg_sq"};
+  static const char* const names8[] = {"exp_avg code", "exp_avg scale", "exp_avg_sq code", "exp_avg_sq scale"};
+  for (int k = 0; k < (eight ? 4 : 2); ++k) {
+    const bool scales = eight && k % 2 == 1;
+    if (!lists.add(eight ? names8[k] : names32[k], PyTuple_GET_ITEM(moments, k), eight && !scales ? kU8 : kF32,
+                   scales ? kScales : kLikeFirst, true, m[k], found))
+      return nullptr;
+  }
+  if (lists.n == 0) return PyLong_FromLong(0);
+  const int code = lists.one_type(p_types, "parameter"), grad_code = code < 0 ? -1 : lists.one_type(g_types, "gradient");
+  if (grad_code < 0) return nullptr;
+  if (grad_code != code && grad_code != MUON_B200_F32)
+    return PyErr_Format(PyExc_ValueError, "%s: gradient tensors must be of the parameters' type or float32", lists.what);
+  if (has_masters && code == MUON_B200_F32)
+    return PyErr_Format(PyExc_ValueError, "%s: float32 parameters have no master weights", lists.what);
+  std::vector<int64_t> steps;
+  if (!read_steps(lists, steps_o, steps)) return nullptr;
+  const float* factor = nullptr;
+  if (scale != Py_None) {
+    const at::Tensor* t = THPVariable_Check(scale) ? &THPVariable_Unpack(scale) : nullptr;
+    if (!t || !t->is_cuda() || t->get_device() != lists.device || t->scalar_type() != at::kFloat || t->numel() != 1)
+      return PyErr_Format(PyExc_ValueError, "%s: grad_scale must be one float32 value on cuda:%lld", lists.what,
+                          (long long)lists.device);
+    factor = static_cast<const float*>(t->const_data_ptr());
+  }
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  void* const* wp = has_masters ? w.data() : nullptr;
+  const int n = static_cast<int>(lists.n);
+  const int rc = eight ? muon_b200_adamw8(p.data(), wp, g.data(), m[0].data(), m[1].data(), m[2].data(), m[3].data(),
+                                          lists.numel.data(), steps.data(), n, code, grad_code, lr, wd, b1, b2, eps, seed,
+                                          factor, stream)
+                       : muon_b200_adamw(p.data(), wp, g.data(), m[0].data(), m[1].data(), lists.numel.data(),
+                                         steps.data(), n, code, grad_code, lr, wd, b1, b2, eps, factor, stream);
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// convert(what, values, codes, scales, kind, to_codes) -> status
+PyObject* convert(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  const char* what;
+  PyObject *values, *codes, *scales;
+  int kind, to_codes;
+  if (!PyArg_ParseTuple(args, "sOOOip", &what, &values, &codes, &scales, &kind, &to_codes)) return nullptr;
+  Lists lists(what);
+  Table x, c, s;
+  int found = 0, types = 0;
+  if (!lists.add("code", codes, kU8, kLikeFirst, to_codes, c, found) ||
+      !lists.add("scale", scales, kF32, kScales, to_codes, s, found) ||
+      !lists.add("value", values, kFloats, kLikeFirst, !to_codes, x, types))
+    return nullptr;
+  if (lists.n == 0) return PyLong_FromLong(0);
+  const int code = lists.one_type(types, "value");
+  if (code < 0) return nullptr;
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const int n = static_cast<int>(lists.n);
+  return PyLong_FromLong(to_codes ? muon_b200_quantize_state(x.data(), c.data(), s.data(), lists.numel.data(), n, code, kind, stream)
+                                  : muon_b200_dequantize_state(c.data(), s.data(), x.data(), lists.numel.data(), n, code, kind, stream));
+  END_HANDLE_TH_ERRORS
+}
+
+// grad_norm(tensors, max_norm, clip, scratch) -> (status, norm, factor). scratch(device) returns the address of
+// muon_b200_grad_norm_scratch_bytes() bytes that this call may use, as an integer.
+PyObject* grad_norm(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *tensors, *scratch;
+  double max_norm;
+  int clip;
+  if (!PyArg_ParseTuple(args, "OdpO", &tensors, &max_norm, &clip, &scratch)) return nullptr;
+  Lists lists(clip ? "clip_grad_norm_" : "grad_norm");
+  Table x;
+  int found = 0;
+  if (!lists.add("gradient", tensors, kFloats, kLikeFirst, clip, x, found)) return nullptr;
+  if (lists.n == 0) return PyErr_Format(PyExc_ValueError, "%s: no tensors", lists.what);
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  Ref held(PyObject_CallFunction(scratch, "LN", (long long)lists.device, PyLong_FromVoidPtr(stream)));
+  if (!held.p) return nullptr;
+  if (!THPVariable_Check(held.p)) return PyErr_Format(PyExc_TypeError, "scratch is no tensor");
+  const at::Tensor& room = THPVariable_Unpack(held.p);
+  const uintptr_t at = (reinterpret_cast<uintptr_t>(room.data_ptr()) + 255) & ~uintptr_t(255);
+  const int64_t bytes = room.numel() - static_cast<int64_t>(at - reinterpret_cast<uintptr_t>(room.data_ptr()));
+  const at::Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, lists.device));
+  const int n = static_cast<int>(lists.n);
+  float* result = out.mutable_data_ptr<float>();
+  const int rc = clip ? muon_b200_clip_grads(x.data(), lists.numel.data(), lists.codes.data(), n, max_norm, result,
+                                             reinterpret_cast<void*>(at), bytes, stream)
+                      : muon_b200_grad_norm(x.data(), lists.numel.data(), lists.codes.data(), n, max_norm, result,
+                                            reinterpret_cast<void*>(at), bytes, stream);
+  return Py_BuildValue("iNN", rc, THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.select(0, 1)));
   END_HANDLE_TH_ERRORS
 }
 
 // gradients(tensors) -> list: parameters give their .grad, other tensors themselves; None is left out.
 PyObject* gradients(PyObject*, PyObject* tensors) {
   HANDLE_TH_ERRORS
-  Ref fast(PySequence_Fast(tensors, "a list of parameters or gradients is wanted")), out(PyList_New(0));
+  Ref fast(PySequence_Fast(tensors, "parameters or gradients are wanted")), out(PyList_New(0));
   if (!fast.p || !out.p) return nullptr;
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.p);
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -181,10 +322,13 @@ PyObject* gradients(PyObject*, PyObject* tensors) {
   END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"gradients", gradients, METH_O, "The gradients of parameters, or the tensors themselves."},
-                         {"collect", collect, METH_VARARGS, "Checks tensor lists and returns their pointer tables."},
-                         {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tables", "Pointer tables of multi-tensor calls.", -1, methods,
+PyMethodDef methods[] = {
+    {"adamw", adamw, METH_VARARGS, "One AdamW step on lists of tensors."},
+    {"convert", convert, METH_VARARGS, "Moments in 32 bits <-> codes and scales."},
+    {"grad_norm", grad_norm, METH_VARARGS, "Norm of a list of tensors and the factor that clips it."},
+    {"gradients", gradients, METH_O, "The gradients of parameters, or the tensors themselves."},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tables", "Multi-tensor calls from lists of tensors.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

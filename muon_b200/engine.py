@@ -13,16 +13,14 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
 from typing import Sequence
 
 import torch
 from torch import Tensor
 
-from . import _lib
-from ._tables import collect
+from . import _lib, _tables
 from ._lib import (BF16, EXP_AVG, EXP_AVG_SQ, F16, F32, F64, NS_AOL4, NS_AOL4_FP8, NS_CLASSIC5, NS_HAVE_SUMSQ,
-                   address, check, i64_array, lib, ptr_array)
+                   check, i64_array, lib, ptr_array)
 
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 # element types the cast at the entry of Newton-Schulz accepts (muon.py:760 takes any float dtype)
@@ -207,28 +205,7 @@ def ramped_sizes(sizes: list[int], growth: float = 0.25) -> list[int]:
     return out
 
 
-# ---- many tensors in one call (AdamW, gradient norm, state conversion) -------------------
 _STATE_KINDS = {"exp_avg": EXP_AVG, "exp_avg_sq": EXP_AVG_SQ}
-# masks of element types as _tables.collect takes them
-_T_F32, _T_U8, _T_FLOATS = 1, 8, 7
-_LIKE_FIRST, _SCALES = 0, 1  # sizes of a list: those of the first list, or one per STATE_BLOCK of its elements
-_current_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _one_type(mask: int, what: str, name: str) -> int:
-    """Element type code of a list whose tensors must all have one type."""
-    if mask & (mask - 1):
-        raise ValueError(f"{what} needs {name} tensors of one dtype")
-    return mask.bit_length() - 1
-
-
-def _call_on(device: int, call, *args) -> None:
-    """A library call with the tensors' device current; the current stream of that device is appended."""
-    if torch.cuda.current_device() == device:
-        check(call(*args, _current_raw_stream(device)))
-    else:
-        with torch.cuda.device(device):
-            check(call(*args, _current_raw_stream(device)))
 
 
 class CudaBackend:
@@ -563,44 +540,17 @@ class CudaBackend:
             self.launch_groups += 1
 
     # -- AdamW, moments in 32 or 8 bits; gradient norm (adamw.py) --------------------------
-    # _tables.collect checks the lists (one device, element types, sizes, memory order, nothing written
-    # twice) and returns their tables of addresses.
-    def _adamw(self, call, what, params, grads, masters, moments, steps, hyper, grad_scale, *seed) -> None:
-        if not params:
-            return
-        lists = [("parameter", params, _T_FLOATS, _LIKE_FIRST, True), ("gradient", grads, _T_FLOATS, _LIKE_FIRST, False)]
-        if masters is not None:
-            lists.append(("master", masters, _T_F32, _LIKE_FIRST, True))
-        device, numel, tables, found, _ = collect(what, (*lists, *moments))
-        code, grad_code = _one_type(found[0], what, "parameter"), _one_type(found[1], what, "gradient")
-        if grad_code != code and grad_code != F32:
-            raise ValueError(f"{what}: gradient tensors must be of the parameters' type or float32")
-        if masters is not None and code == F32:
-            raise ValueError(f"{what}: float32 parameters have no master weights")
-        n = len(params)
-        steps = array("q", [steps]) * n if isinstance(steps, int) else array("q", steps)
-        if len(steps) != n:
-            raise ValueError(f"{what}: {len(steps)} steps for {n} tensors")
-        factor = None
-        if grad_scale is not None:
-            if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != device:
-                raise ValueError(f"{what}: grad_scale must be one float32 value on cuda:{device}")
-            factor = grad_scale.data_ptr()
-        if _grad_ready:
-            _wait_grads(torch.cuda.current_stream(device), grads)
-        p, g = tables[:2]
-        w, rest = (None, tables[2:]) if masters is None else (tables[2], tables[3:])
-        _call_on(device, call, p, w, g, *rest, numel, address(steps), n, code, grad_code, *hyper, *seed, factor)
-        self.launch_groups += 1
-
+    # _tables checks the lists (one device, element types, sizes, memory order, nothing written twice) and
+    # makes the library call on the current stream of their device.
     def adamw_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                    exp_avg_sqs: Sequence[Tensor], steps, lr: float, weight_decay: float, betas: tuple[float, float],
                    eps: float, masters=None, grad_scale: Tensor | None = None) -> None:
         """AdamW with float32 moments on tensors of any sizes; one parameter and one gradient dtype."""
-        self._adamw(lib.muon_b200_adamw, "adamw_step", params, grads, masters,
-                    (("exp_avg", exp_avgs, _T_F32, _LIKE_FIRST, True),
-                     ("exp_avg_sq", exp_avg_sqs, _T_F32, _LIKE_FIRST, True)),
-                    steps, (lr, weight_decay, betas[0], betas[1], eps), grad_scale)
+        if _grad_ready and grads:
+            _wait_grads(torch.cuda.current_stream(grads[0].device), grads)
+        check(_tables.adamw(params, grads, masters, (exp_avgs, exp_avg_sqs), steps, lr, weight_decay, betas[0], betas[1],
+                            eps, grad_scale, 0))
+        self.launch_groups += 1
 
     def adamw8_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg_codes: Sequence[Tensor],
                     exp_avg_scales: Sequence[Tensor], exp_avg_sq_codes: Sequence[Tensor],
@@ -608,46 +558,38 @@ class CudaBackend:
                     betas: tuple[float, float], eps: float, masters=None, grad_scale: Tensor | None = None,
                     seed: int = 0) -> None:
         """AdamW with moments in 8 bits (codes of the parameter's size, one float32 scale per 256)."""
-        self._adamw(lib.muon_b200_adamw8, "adamw8_step", params, grads, masters,
-                    (("exp_avg code", exp_avg_codes, _T_U8, _LIKE_FIRST, True),
-                     ("exp_avg scale", exp_avg_scales, _T_F32, _SCALES, True),
-                     ("exp_avg_sq code", exp_avg_sq_codes, _T_U8, _LIKE_FIRST, True),
-                     ("exp_avg_sq scale", exp_avg_sq_scales, _T_F32, _SCALES, True)),
-                    steps, (lr, weight_decay, betas[0], betas[1], eps), grad_scale, seed & 0xFFFFFFFF)
-
-    def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> Tensor:
-        """{norm, factor} of all `tensors` together, on their device; with `clip` the tensors are
-        multiplied by the factor."""
-        what = "clip_grad_norm_" if clip else "grad_norm"
-        device, numel, tables, _, codes = collect(what, (("gradient", tensors, _T_FLOATS, _LIKE_FIRST, clip),))
-        if _grad_ready:
-            _wait_grads(torch.cuda.current_stream(device), tensors)
-        out = torch.empty(2, dtype=torch.float32, device=tensors[0].device)
-        need = lib.muon_b200_grad_norm_scratch_bytes()
-        key = (device, _current_raw_stream(device), 5)
-        if torch.cuda.is_current_stream_capturing():
-            # A captured call gets scratch of its own, from the graph's memory: two graphs captured on
-            # one stream may be replayed at the same time on two.
-            scratch = torch.empty(need + 256, dtype=torch.uint8, device=out.device)
-        elif (scratch := self._workspaces.get(key)) is None:
-            scratch = self.workspace(out.device, need, slot=5)
-        _call_on(device, lib.muon_b200_clip_grads if clip else lib.muon_b200_grad_norm, tables[0], numel, codes,
-                 len(tensors), max_norm, out.data_ptr(), self._aligned_ptr(scratch), need)
+        if _grad_ready and grads:
+            _wait_grads(torch.cuda.current_stream(grads[0].device), grads)
+        check(_tables.adamw(params, grads, masters, (exp_avg_codes, exp_avg_scales, exp_avg_sq_codes, exp_avg_sq_scales),
+                            steps, lr, weight_decay, betas[0], betas[1], eps, grad_scale, seed & 0xFFFFFFFF))
         self.launch_groups += 1
-        return out
+
+    def _norm_scratch(self, device: int, stream: int) -> Tensor:
+        """Scratch of a norm on `stream`, called with `device` current. A captured call gets its own, from the
+        graph's memory: two graphs captured on one stream may be replayed at the same time on two."""
+        captured = torch.cuda.is_current_stream_capturing()
+        buf = None if captured else self._workspaces.get((device, stream, 5))
+        if buf is None:
+            buf = torch.empty(lib.muon_b200_grad_norm_scratch_bytes() + 256, dtype=torch.uint8,
+                              device=torch.device("cuda", device))
+            if not captured:
+                self._workspaces[(device, stream, 5)] = buf
+        return buf
+
+    def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> tuple[Tensor, Tensor]:
+        """(norm, factor) of all `tensors` together, on their device; with `clip` the tensors are
+        multiplied by the factor."""
+        if _grad_ready:
+            _wait_grads(torch.cuda.current_stream(tensors[0].device), tensors)
+        rc, norm, factor = _tables.grad_norm(tensors, max_norm, clip, self._norm_scratch)
+        check(rc)
+        self.launch_groups += 1
+        return norm, factor
 
     def convert_state(self, what: str, values: Sequence[Tensor], codes: Sequence[Tensor], scales: Sequence[Tensor],
                       kind: str, to_codes: bool) -> None:
         """Values <-> 8-bit codes and scales, one dtype of values per call."""
-        if not codes:
-            return
-        device, numel, (c, s, x), found, _ = collect(what, (
-            ("code", codes, _T_U8, _LIKE_FIRST, to_codes), ("scale", scales, _T_F32, _SCALES, to_codes),
-            ("value", values, _T_FLOATS, _LIKE_FIRST, not to_codes)))
-        code = _one_type(found[2], what, "value")
-        tables = (x, c, s) if to_codes else (c, s, x)
-        _call_on(device, lib.muon_b200_quantize_state if to_codes else lib.muon_b200_dequantize_state, *tables, numel,
-                 len(codes), code, _STATE_KINDS[kind])
+        check(_tables.convert(what, values, codes, scales, _STATE_KINDS[kind], to_codes))
         self.launch_groups += 1
 
     # -- functional pieces -------------------------------------------------------------

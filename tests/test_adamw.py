@@ -60,7 +60,7 @@ def test_random_bits_are_uniform_and_uncorrelated():
 
 def _call(name, *tables_then_scalars):
     import muon_b200._lib as L
-    keep = [L.address(x) if isinstance(x, array) else x for x in tables_then_scalars]
+    keep = [x.buffer_info()[0] if isinstance(x, array) else x for x in tables_then_scalars]
     rc = getattr(L.lib, name)(*keep)
     return rc, L.lib.muon_b200_last_error().decode()
 
@@ -111,17 +111,22 @@ def test_no_cpu_fallback():
             call()
 
 
-def test_pointer_tables_refuse_what_is_no_cuda_tensor():
-    from muon_b200._tables import collect
+def test_lists_refuse_what_is_no_cuda_tensor():
+    import muon_b200 as mb
     with pytest.raises(RuntimeError, match="every gradient tensor of grad_norm .* no CPU implementation"):
-        collect("grad_norm", (("gradient", [torch.zeros(3)], 7, 0, False),))
-    for bad in ([1], [None], [[torch.zeros(1)]]):
+        mb.grad_norm([torch.zeros(3)])
+    for bad in ([1], [[torch.zeros(1)]], ["x"]):
         with pytest.raises(TypeError, match="is no tensor"):
-            collect("grad_norm", (("gradient", bad, 7, 0, False),))
-    with pytest.raises(TypeError):
-        collect("grad_norm", (("gradient", 5, 7, 0, False),))
-    device, numel, tables, found, codes = collect("grad_norm", (("gradient", [], 7, 0, False),))
-    assert (device, numel, tables, found, codes) == (-1, b"", (b"",), (0,), b"")
+            mb.grad_norm(bad)
+    for bad in (5, None):
+        with pytest.raises(TypeError):
+            mb.clip_grad_norm_(bad, 1.0)
+    assert [float(x) for x in mb.grad_norm([None])] == [0.0, 1.0] and float(mb.clip_grad_norm_([], 1.0)) == 0.0
+    mb.adamw_step([], [], [], [], 1)
+    mb.adamw8_step([], [], [], [], [], [], [])
+    with pytest.raises(ValueError, match="1 gradient tensors for 0"):
+        mb.adamw_step([], [torch.zeros(1)], [], [], 1)
+    assert mb.dequantize_state([], [], "exp_avg") == []
 
 
 # ------------------------------------------------------------------------------- the classes, without a GPU
@@ -160,7 +165,7 @@ class _OracleBackend:
 
     def grad_norm(self, tensors, max_norm, clip):
         norm = math.sqrt(sum(float(t.double().square().sum()) for t in tensors))
-        return torch.tensor([norm, min(1.0, max_norm / (norm + 1e-6))])
+        return torch.tensor(norm), torch.tensor(min(1.0, max_norm / (norm + 1e-6)))
 
     def convert_state(self, what, values, codes, scales, kind, to_codes):
         for x, c, s in zip(values, codes, scales):
