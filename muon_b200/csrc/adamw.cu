@@ -210,9 +210,11 @@ struct AdamW32Args {
 
 template <typename P>
 constexpr int kVec32 = sizeof(P) == 4 ? 4 : 8;
-constexpr int kIters32 = 4;
+// One vector a thread and no loop: four streams in and three out keep enough bytes in flight by themselves,
+// and short-lived blocks leave no tail. Four layers of bf16 weights, 872M: 2791 us, 2826, 2859, 2914 with 1, 2, 4, 8
+// vectors a thread; 128 float32 filters, 47M: 193, 196, 200, 203.
 template <typename P>
-constexpr int kChunk32 = kThreads * kVec32<P> * kIters32;
+constexpr int kChunk32 = kThreads * kVec32<P>;
 
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads)
@@ -241,8 +243,8 @@ adamw32_kernel(const __grid_constant__ AdamW32Args<CAP> a) {
   int done = 0;  // elements of the chunk that the vector loop covers
   if (a.head[t] != kNoHead) {
     done = left >= kChunk32<P> ? kChunk32<P> : (int)left / V * V;
-#pragma unroll 2
-    for (int i = threadIdx.x * V; i < done; i += kThreads * V) {
+    const int i = threadIdx.x * V;
+    if (i < done) {
       Raw<P, V> rp;
       Raw<float, V> rw, rm, rv;
       Raw<G, V> rg;
