@@ -6,6 +6,7 @@
 #include "ns_gemm.h"
 #include "profiling.h"
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -865,29 +866,40 @@ __device__ __forceinline__ double block_sum(double v, double (&warps)[kWarps]) {
 }
 
 template <int CAP>
+__device__ __forceinline__ double squares_of(const NormArgs<CAP>& a, int chunk) {
+  const int t = find_tensor(a.start, a.count, chunk);
+  const int k = chunk - a.start[t], head = a.head[t];
+  const long long n = a.numel[t];
+  if (a.dtype[t] == DT_F32) return chunk_squares(static_cast<const float*>(a.x[t]), k, head, n);
+  if (a.dtype[t] == DT_BF16) return chunk_squares(static_cast<const __nv_bfloat16*>(a.x[t]), k, head, n);
+  return chunk_squares(static_cast<const __half*>(a.x[t]), k, head, n);
+}
+
+template <int CAP>
 __global__ void __launch_bounds__(kThreads, kNormBlocksPerSm)
 norm_partial_kernel(const __grid_constant__ NormArgs<CAP> a) {
   __shared__ double warps[kWarps];
   double acc = 0.0;
-  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-    const int t = find_tensor(a.start, a.count, chunk);
-    const int k = chunk - a.start[t], head = a.head[t];
-    const long long n = a.numel[t];
-    if (a.dtype[t] == DT_F32) acc += chunk_squares(static_cast<const float*>(a.x[t]), k, head, n);
-    else if (a.dtype[t] == DT_BF16) acc += chunk_squares(static_cast<const __nv_bfloat16*>(a.x[t]), k, head, n);
-    else acc += chunk_squares(static_cast<const __half*>(a.x[t]), k, head, n);
-  }
+  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) acc += squares_of(a, chunk);
   acc = block_sum(acc, warps);
   if (threadIdx.x == 0) a.partials[blockIdx.x] = acc;
 }
 
-// {norm, factor} from the partial sums: every block that needs them adds them up in the same order.
+// {norm, factor that clips}; a NaN stays.
+__device__ __forceinline__ float2 norm_and_factor(double sum, float max_norm) {
+  const float norm = (float)sqrt(sum), q = max_norm / (norm + 1e-6f);
+  return make_float2(norm, q > 1.f ? 1.f : q);
+}
+// The factor that grad_norm hands out: none where the norm is not finite.
+__device__ __forceinline__ float handed_out(float2 r) {
+  return fabsf(r.x) <= 3.402823466e38f ? r.y : __int_as_float(0x7fffffff);
+}
+
+// From the partial sums: every block that needs the result adds them up in the same order.
 __device__ __forceinline__ float2 finish_norm(const double* partials, int n, float max_norm, double (&warps)[kWarps]) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < n; i += kThreads) acc += partials[i];
-  const float norm = (float)sqrt(block_sum(acc, warps));
-  const float q = max_norm / (norm + 1e-6f);
-  return make_float2(norm, q > 1.f ? 1.f : q);  // a NaN stays
+  return norm_and_factor(block_sum(acc, warps), max_norm);
 }
 
 __global__ void __launch_bounds__(kThreads)
@@ -896,7 +908,7 @@ norm_finish_kernel(const double* partials, int n, float max_norm, float* out2) {
   const float2 r = finish_norm(partials, n, max_norm, warps);
   if (threadIdx.x == 0) {
     out2[0] = r.x;
-    out2[1] = fabsf(r.x) <= 3.402823466e38f ? r.y : __int_as_float(0x7fffffff);
+    out2[1] = handed_out(r);
   }
 }
 
@@ -923,6 +935,16 @@ __device__ __forceinline__ void scale_chunk(T* x, int chunk, int head, long long
 }
 
 template <int CAP>
+__device__ __forceinline__ void scale_one(const NormArgs<CAP>& a, int chunk, float f) {
+  const int t = find_tensor(a.start, a.count, chunk);
+  const int k = chunk - a.start[t], head = a.head[t];
+  const long long n = a.numel[t];
+  if (a.dtype[t] == DT_F32) scale_chunk(static_cast<float*>(a.x[t]), k, head, n, f);
+  else if (a.dtype[t] == DT_BF16) scale_chunk(static_cast<__nv_bfloat16*>(a.x[t]), k, head, n, f);
+  else scale_chunk(static_cast<__half*>(a.x[t]), k, head, n, f);
+}
+
+template <int CAP>
 __global__ void __launch_bounds__(kThreads)
 clip_kernel(const __grid_constant__ NormArgs<CAP> a, int partials, float max_norm, float* out2) {
   __shared__ double warps[kWarps];
@@ -931,15 +953,40 @@ clip_kernel(const __grid_constant__ NormArgs<CAP> a, int partials, float max_nor
     out2[0] = r.x;
     out2[1] = r.y;
   }
-  const float f = r.y;
-  if (f == 1.f) return;  // nothing to clip: x * 1 is x
-  for (int chunk = a.chunks - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) {
-    const int t = find_tensor(a.start, a.count, chunk);
-    const int k = chunk - a.start[t], head = a.head[t];
-    const long long n = a.numel[t];
-    if (a.dtype[t] == DT_F32) scale_chunk(static_cast<float*>(a.x[t]), k, head, n, f);
-    else if (a.dtype[t] == DT_BF16) scale_chunk(static_cast<__nv_bfloat16*>(a.x[t]), k, head, n, f);
-    else scale_chunk(static_cast<__half*>(a.x[t]), k, head, n, f);
+  if (r.y == 1.f) return;  // nothing to clip: x * 1 is x
+  // from the end: what the norm's pass read last is still in L2
+  for (int chunk = a.chunks - 1 - (int)blockIdx.x; chunk >= 0; chunk -= gridDim.x) scale_one(a, chunk, r.y);
+}
+
+// The whole of a call with few chunks in one launch of one cluster: the blocks' sums meet in shared memory
+// instead of global memory, and each block scales what it summed. For 25 vectors of 768 a call returns after
+// 7.6 instead of 10.5 us (a launch less), while the device takes 4.0 instead of 3.1 us.
+constexpr int kClusterBlocks = 8, kClusterChunks = 32;
+
+template <int CAP, bool CLIP>
+__global__ void __cluster_dims__(kClusterBlocks) __launch_bounds__(kThreads)
+norm_cluster_kernel(const __grid_constant__ NormArgs<CAP> a, float max_norm, float* out2) {
+  namespace cg = cooperative_groups;
+  __shared__ double warps[kWarps];
+  __shared__ double mine;
+  const cg::cluster_group cluster = cg::this_cluster();
+  double acc = 0.0;
+  for (int chunk = blockIdx.x; chunk < a.chunks; chunk += kClusterBlocks) acc += squares_of(a, chunk);
+  acc = block_sum(acc, warps);
+  if (threadIdx.x == 0) mine = acc;
+  cluster.sync();
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < kClusterBlocks; ++k) sum += *cluster.map_shared_rank(&mine, k);
+  cluster.sync();  // no block leaves while its sum is read
+  const float2 r = norm_and_factor(sum, max_norm);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    out2[0] = r.x;
+    out2[1] = CLIP ? r.y : handed_out(r);
+  }
+  if constexpr (CLIP) {
+    if (r.y == 1.f) return;
+    for (int chunk = blockIdx.x; chunk < a.chunks; chunk += kClusterBlocks) scale_one(a, chunk, r.y);
   }
 }
 
@@ -1262,6 +1309,25 @@ int grad_norm_partials(int* n) {
 }
 
 namespace {
+// A call with few chunks as one launch. False: it has more (or none), and nothing was launched.
+template <bool CLIP>
+int norm_in_one_launch(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
+                       float* out2, cudaStream_t stream, bool* done) {
+  *done = false;
+  if (count > kCapFew) return OK;
+  return for_each_norm_table<kCapFew>(
+      tensors, numel, dtypes, count, nullptr, [&](NormArgs<kCapFew>& a, double bytes) -> int {
+        int sms = 0;
+        const int rc = device_sm_count(&sms);
+        if (rc != OK || a.chunks > kClusterChunks) return rc;
+        *done = true;  // (the lists of up to kCapFew tensors with so few chunks are one table)
+        LaunchScope scope(K_GRAD_NORM, CLIP ? 3.0 * bytes : bytes, stream);
+        norm_cluster_kernel<kCapFew, CLIP><<<kClusterBlocks, kThreads, 0, stream>>>(a, (float)max_norm, out2);
+        MB_CUDA_CHECK(cudaGetLastError());
+        return OK;
+      });
+}
+
 template <int CAP>
 int clip_launch(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
                 float* out2, double* partials, cudaStream_t stream) {
@@ -1289,9 +1355,11 @@ int clip_launch(void* const* tensors, const int64_t* numel, const int* dtypes, i
 
 int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
                   float* out2, double* partials, cudaStream_t stream) {
-  int n = 0;
-  const int rc = count <= kCapFew ? norm_partials<kCapFew>(tensors, numel, dtypes, count, partials, &n, stream)
-                                  : norm_partials<kCapNorm>(tensors, numel, dtypes, count, partials, &n, stream);
+  bool done = false;
+  int n = 0, rc = norm_in_one_launch<false>(tensors, numel, dtypes, count, max_norm, out2, stream, &done);
+  if (rc != OK || done) return rc;
+  rc = count <= kCapFew ? norm_partials<kCapFew>(tensors, numel, dtypes, count, partials, &n, stream)
+                        : norm_partials<kCapNorm>(tensors, numel, dtypes, count, partials, &n, stream);
   if (rc != OK) return rc;
   LaunchScope scope(K_GRAD_NORM, 8.0 * n, stream);
   norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, n, (float)max_norm, out2);
@@ -1301,6 +1369,9 @@ int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes,
 
 int run_clip(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
              float* out2, double* partials, cudaStream_t stream) {
+  bool done = false;
+  const int rc = norm_in_one_launch<true>(tensors, numel, dtypes, count, max_norm, out2, stream, &done);
+  if (rc != OK || done) return rc;
   return count <= kCapFew ? clip_launch<kCapFew>(tensors, numel, dtypes, count, max_norm, out2, partials, stream)
                           : clip_launch<kCapNorm>(tensors, numel, dtypes, count, max_norm, out2, partials, stream);
 }

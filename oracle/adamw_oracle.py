@@ -71,10 +71,14 @@ def quantize(x: torch.Tensor, kind: str, bits=None):
 
 
 def random_bits(n: int, seed: int, step: int) -> torch.Tensor:
-    """The 20 random bits of elements 0 .. n-1 of a tensor (32-bit arithmetic in Python integers for
-    the key, in int64 tensors for the rest)."""
+    """The 20 random bits of elements 0 .. n-1 of a tensor."""
+    return random_bits_at(torch.arange(n, dtype=torch.int64), seed, step)
+
+
+def random_bits_at(i: torch.Tensor, seed: int, step: int) -> torch.Tensor:
+    """The same for the elements of these indexes (32-bit arithmetic in Python integers for the key, in
+    int64 tensors for the rest)."""
     mod = 1 << 32
-    i = torch.arange(n, dtype=torch.int64)
     key = (seed * 0x3C6EF373 + step * 0xBB67AE85) % mod
     h = ((i // 4) * 0x9E3779B1 + key) % mod
     h = ((h ^ (h >> 16)) * 0x6A09E667) % mod

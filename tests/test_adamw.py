@@ -358,3 +358,32 @@ def test_auxiliary_adam_keeps_other_moments_when_asked(backend):
                 for to in (target, other):
                     got = to.state[p][key]
                     assert (got.dtype == value.dtype and torch.equal(got, value)) if torch.is_tensor(value) else got == value
+
+
+def test_adamw_class_on_dtensors(backend, tmp_path):
+    """Row-sharded parameters on a mesh of one rank: the local part is stepped, with moments of its own; a
+    gradient in another placement is brought into the parameter's; clipping is refused."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Partial, Shard
+    import muon_b200 as mb
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/pg", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        gen = torch.Generator().manual_seed(8)
+        w, g = torch.randn(70, 80, generator=gen), torch.randn(70, 80, generator=gen)
+        p = torch.nn.Parameter(DTensor.from_local(w.clone(), mesh, [Shard(0)]))
+        q = torch.nn.Parameter(w.clone())
+        ours, plain = mb.AdamW([p], state_bits=8), mb.AdamW([q], state_bits=8)
+        for placement in (Shard(0), Partial()):
+            p.grad = DTensor.from_local(g.clone(), mesh, [placement])
+            q.grad = g.clone()
+            ours.step()
+            plain.step()
+        assert torch.equal(p.to_local(), q) and ours.state[p]["exp_avg_codes"].shape == (70, 80)
+        assert torch.equal(ours.state[p]["exp_avg_codes"], plain.state[q]["exp_avg_codes"])
+        clipped = mb.AdamW([p], max_grad_norm=1.0)
+        with pytest.raises(ValueError, match="whole gradients"):
+            clipped.step()
+    finally:
+        dist.destroy_process_group()

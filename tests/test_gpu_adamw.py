@@ -278,11 +278,12 @@ def _norm_error(n):
     return (4 + 1) * 2.0 ** -24
 
 
+@pytest.mark.parametrize("times", [1, 3, 9], ids=["few", "some", "many"])  # one launch, and both sizes of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
-def test_grad_norm_and_clip(mb, offset):
+def test_grad_norm_and_clip(mb, offset, times):
     gen = torch.Generator().manual_seed(12)
     kinds = [torch.float32, torch.bfloat16, torch.float16]
-    g = [(torch.randn(n, generator=gen) * 3).to(kinds[i % 3]) for i, n in enumerate(SIZES)]
+    g = [(torch.randn(n, generator=gen) * 3).to(kinds[i % 3]) for i, n in enumerate(SIZES * times + [100003] * (times - 1))]
     G = [_place([x], x.dtype, offset)[0] for x in g]
     exact = math.sqrt(sum(float(x.double().square().sum()) for x in g))
     norm, factor = mb.grad_norm(G, 2.0)
@@ -329,6 +330,41 @@ def test_norm_of_parameters_and_of_nothing(mb):
     assert q.grad is None and float(p.grad.norm()) == pytest.approx(1.0, rel=1e-5)
     assert float(mb.clip_grad_norm_([q], 1.0)) == 0.0 and float(mb.grad_norm([q])[1]) == 1.0
     assert float(mb.clip_grad_norm_([torch.zeros(0, device="cuda")], 1.0)) == 0.0
+
+
+def test_elements_past_32_bits(mb):
+    """2^32 + 300 elements of bfloat16: the last ones are stepped, summed, scaled and expanded like others."""
+    n, tail = (1 << 32) + 300, 700  # the last blocks, from a multiple of 256 on
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    first = (n - tail) // 256 * 256
+    gen = torch.Generator().manual_seed(30)
+    p, g = (torch.randn(n - first, generator=gen) * 0.02).bfloat16(), (torch.randn(n - first, generator=gen) * 0.01).bfloat16()
+    P, G = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    P[first:], G[first:] = p.cuda(), g.cuda()
+    codes = [torch.zeros(n, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(-(-n // 256), device="cuda") for _ in range(2)]
+    norm, factor = mb.grad_norm([G], 0.01)
+    exact = float(g.double().norm())
+    assert abs(float(norm) - exact) <= _norm_error(0) * exact
+    mb.adamw8_step([P], [G], codes[:1], scales[:1], codes[1:], scales[1:], 1, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD,
+                   grad_scale=factor, seed=3)
+    zeros = torch.zeros(n - first)
+    f = float(factor)
+    m, v = orc.moments32(g, zeros, zeros, BETAS, f)
+    index = torch.arange(n - first) + first  # the hash is taken of the low 32 bits of index / 4: 2^32 / 4 is within
+    bits = orc.random_bits_at(index, 3, 1)
+    for k, (x, kind, r) in enumerate(((m, "exp_avg", None), (v, "exp_avg_sq", bits))):
+        _check_codes(codes[k][first:], scales[k][first // 256:], orc.quantize(x, kind, r), kind, kind)
+        out = mb.dequantize_state(codes[k:k + 1], scales[k:k + 1], kind, dtype=torch.bfloat16)[0]
+        assert torch.equal(out[first:].cpu(), orc.dequantize(codes[k][first:].cpu(), scales[k][first // 256:].cpu(), kind).bfloat16())
+        assert (out[:256] == 0).all() and (out[first - 512:first] == 0).all()
+        del out
+    args = (p, g, zeros, zeros, 1, LR, BETAS, EPS, WD, f)
+    want = orc.adamw64(*args)[0]
+    _assert_close(P[first:], want, orc.adamw_tolerance(*args)[0] + _half_step(want, torch.bfloat16), "parameter")
+    assert torch.equal(mb.clip_grad_norm_([G], 0.01), norm)
+    assert torch.equal(G[first:].cpu(), (g.float() * factor.cpu()).bfloat16()) and (G[:first] == 0).all()
 
 
 # ------------------------------------------------------------------------------------ conversion
