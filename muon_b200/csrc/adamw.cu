@@ -360,7 +360,7 @@ __device__ __forceinline__ uint32_t pack_bytes(int b1, int b0, uint32_t high) {
 
 // Eight codes of a moment <-> floats.
 template <int KIND>
-__device__ __forceinline__ void decode8(uint2 w, float scale, float2 (&x)[4]) {
+__device__ __forceinline__ void decode8(uint2 w, float2 (&x)[4]) {  // in units of the scale
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const uint32_t u = h ? w.y : w.x;
@@ -372,9 +372,12 @@ __device__ __forceinline__ void decode8(uint2 w, float scale, float2 (&x)[4]) {
       x[2 * h + 1] = make_float2(sq_value<2>(u), sq_value<3>(u));
     }
   }
-  const float2 s = make_float2(scale, scale);
+}
+template <int KIND>
+__device__ __forceinline__ void decode8(uint2 w, float scale, float2 (&x)[4]) {
+  decode8<KIND>(w, x);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], s);
+  for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], both(scale));
 }
 template <int KIND>
 __device__ __forceinline__ uint2 encode8(const float2 (&x)[4], float inv, const uint32_t (&r)[8]) {
@@ -671,7 +674,7 @@ struct ConvertArgs {
   float* scales[CAP];
   long long numel[CAP];
   int start[CAP + 1];
-  unsigned char vec_ok[CAP];
+  unsigned char head[CAP];  // first element aligned in both lists (quantize: 0), or kNoHead
   int count;
   uint32_t half;  // half a code (2^19), added before the cut: to nearest
 };
@@ -695,7 +698,7 @@ quantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
     if (b >= blocks) return;
     const long long base = b * kStateBlock;
     const long long at = base + lane * 8;
-    const bool vec = a.vec_ok[t] && base + kStateBlock <= numel;
+    const bool vec = a.head[t] == 0 && base + kStateBlock <= numel;
     float2 xj[4];
     if (vec) {
       Raw<T, 8> rx;
@@ -723,56 +726,66 @@ quantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
   }
 }
 
-// A warp expands four consecutive blocks: 16 codes a lane from two blocks at a time, so that codes are
-// read and values written 16 bytes and more to a lane.
+// A warp expands 1024 consecutive elements, 16 codes a lane at a time, so that codes are read and values
+// written 16 bytes and more to a lane. It starts where codes and values are both aligned; 16 codes from
+// there may lie in two blocks.
 template <typename T, int KIND, int CAP>
 __global__ void __launch_bounds__(kThreads)
 dequantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
+  constexpr int kPieces = kBlocksPerWarp / 2, kSpan = kBlocksPerWarp * kStateBlock;
   const int t = find_tensor(a.start, a.count, (int)blockIdx.x);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long numel = a.numel[t];
   T* x = static_cast<T*>(a.x[t]);
   const uint8_t* codes = a.codes[t];
   const float* scales = a.scales[t];
-  const long long b0 = ((long long)((int)blockIdx.x - a.start[t]) * kWarps + warp) * kBlocksPerWarp;
-  const long long base = b0 * kStateBlock;
+  const bool vec = a.head[t] != kNoHead;
+  const int head = vec ? a.head[t] : 0;
+  const long long task = (long long)((int)blockIdx.x - a.start[t]) * kWarps + warp, base = task * kSpan + head;
+  const auto single = [&](long long i) { x[i] = from_float<T>(decode1<KIND>(codes[i], scales[i / kStateBlock])); };
+  if (task == 0 && lane < head) single(lane);
   if (base >= numel) return;
-  if (a.vec_ok[t]) {
-    constexpr int kPieces = kBlocksPerWarp / 2;
-    uint4 c[kPieces];
-    float scale[kPieces];
-#pragma unroll
-    for (int k = 0; k < kPieces; ++k) {
-      const long long at = base + 2 * k * kStateBlock + 16 * lane;
-      if (at >= numel) continue;
-      scale[k] = scales[b0 + 2 * k + (lane >> 4)];
-      if (at + 16 <= numel) c[k] = __ldcs(reinterpret_cast<const uint4*>(codes + at));
-    }
-#pragma unroll
-    for (int k = 0; k < kPieces; ++k) {
-      const long long at = base + 2 * k * kStateBlock + 16 * lane;
-      if (at + 16 <= numel) {
-        float2 lo[4], hi[4], all[8];
-        decode8<KIND>(make_uint2(c[k].x, c[k].y), scale[k], lo);
-        decode8<KIND>(make_uint2(c[k].z, c[k].w), scale[k], hi);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          all[j] = lo[j];
-          all[4 + j] = hi[j];
-        }
-        Raw<T, 16> rx;
-        rx.pack(all);
-        rx.store(x + at);
-      } else {
-        for (long long i = at; i < numel; ++i) x[i] = from_float<T>(decode1<KIND>(codes[i], scale[k]));
-      }
-    }
+  if (!vec) {
+    const int n = (int)min(numel - base, (long long)kSpan);
+#pragma unroll 8
+    for (int i = lane; i < n; i += 32) single(base + i);
     return;
   }
-  const int n = (int)min(numel - base, (long long)kBlocksPerWarp * kStateBlock);
-#pragma unroll 8
-  for (int i = lane; i < n; i += 32)
-    x[base + i] = from_float<T>(decode1<KIND>(codes[base + i], scales[b0 + i / kStateBlock]));
+  uint4 c[kPieces];
+  float first[kPieces], second[kPieces];
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const long long at = base + 512 * k + 16 * lane;
+    if (at + 16 <= numel) {
+      c[k] = __ldcs(reinterpret_cast<const uint4*>(codes + at));
+      first[k] = scales[at / kStateBlock];
+      second[k] = scales[(at + 15) / kStateBlock];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const long long at = base + 512 * k + 16 * lane;
+    if (at + 16 <= numel) {
+      const int split = kStateBlock - (int)(at % kStateBlock);  // elements before the second block
+      float2 lo[4], hi[4], all[8];
+      decode8<KIND>(make_uint2(c[k].x, c[k].y), lo);
+      decode8<KIND>(make_uint2(c[k].z, c[k].w), hi);
+      if (split >= 16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) all[j] = mul2(j < 4 ? lo[j & 3] : hi[j & 3], both(first[k]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          all[j] = mul2(j < 4 ? lo[j & 3] : hi[j & 3], make_float2(2 * j < split ? first[k] : second[k],
+                                                                 2 * j + 1 < split ? first[k] : second[k]));
+      }
+      Raw<T, 16> rx;
+      rx.pack(all);
+      rx.store(x + at);
+    } else {
+      for (long long i = at; i < numel; ++i) single(i);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1240,7 +1253,17 @@ int convert_launch(void* const* x, void* const* codes, void* const* scales, cons
   a.start[0] = 0;
   for (int i = 0; i <= count; ++i) {
     const int64_t per = (int64_t)kBlocksPerChunk * kStateBlock;
-    const int64_t chunks = i < count ? (numel[i] + per - 1) / per : 0;
+    int head = 0;
+    int64_t chunks = 0;
+    if (i < count && numel[i] > 0) {
+      if (TO_CODES) {  // (its blocks start at the tensor's first element)
+        head = aligned(x[i], 8 * sizeof(T)) && aligned(codes[i], 8) ? 0 : kNoHead;
+      } else {
+        head = common_head<16>({{x[i], sizeof(T)}, {codes[i], 1}});
+        if (head > numel[i]) head = kNoHead;
+      }
+      chunks = (numel[i] + per - 1) / per;  // (a head only makes the last chunk shorter)
+    }
     if (i == count || n == CAP || !fits(a.start[n], chunks)) {
       if (n > 0) {
         a.count = n;
@@ -1257,7 +1280,7 @@ int convert_launch(void* const* x, void* const* codes, void* const* scales, cons
     a.codes[n] = static_cast<uint8_t*>(codes[i]);
     a.scales[n] = static_cast<float*>(scales[i]);
     a.numel[n] = numel[i];
-    a.vec_ok[n] = aligned(x[i], TO_CODES ? 8 * sizeof(T) : 32) && aligned(codes[i], TO_CODES ? 8 : 16);
+    a.head[n] = (unsigned char)head;
     a.start[n + 1] = a.start[n] + (int)chunks;
     elems += (double)numel[i];
     ++n;

@@ -148,6 +148,83 @@ def test_adamw8_step(mb, dtype, master, offset):
                 _assert_close(P[i], want, tol + _half_step(want, t), f"parameter {n}")
 
 
+class _Guarded:
+    """Copies on the device with 64 other elements on either side, `offset` elements behind a boundary."""
+
+    def __init__(self, ts, dtype, offset):
+        self.bufs = [torch.full((t.numel() + 128 + offset,), 77, dtype=dtype, device="cuda") for t in ts]
+        self.views = [b[64 + offset:64 + offset + t.numel()] for b, t in zip(self.bufs, ts)]
+        self.offset = offset
+        for v, t in zip(self.views, ts):
+            v.copy_(t)
+
+    def intact(self):
+        return all((b[:64 + self.offset] == 77).all() and (b[len(b) - 64:] == 77).all() for b in self.bufs)
+
+
+@pytest.mark.parametrize("offsets", [(1, 3, 2, 5, 7), (7, 7, 7, 7, 7), (0, 0, 1, 0, 0), (4, 2, 8, 13, 3), (0, 5, 0, 0, 2)])
+@pytest.mark.parametrize("master", [False, True], ids=["plain", "master"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_lists_that_start_anywhere(mb, dtype, master, offsets):
+    """Every list at another distance from a 16-byte boundary, both steps: results as defined, and nothing
+    beside the tensors is touched."""
+    t = DTYPES[dtype]
+    if t == torch.float32 and master:
+        pytest.skip("float32 parameters have no masters")
+    sizes = [15, 256, 271, 272, 273, 512, 528, 530, 256 * 40 + 100, 20001]
+    p, g, m, v = _inputs(sizes, 40, t)
+    w = [x.float() for x in p] if master else None
+    po, go, mo, vo, wo = offsets
+    P, G = _Guarded(p, t, po), _Guarded(g, t, go)
+    W = _Guarded(w, torch.float32, wo) if master else None
+    # float32 moments
+    M, V = _Guarded(m, torch.float32, mo), _Guarded(v, torch.float32, vo)
+    mb.adamw_step(P.views, G.views, M.views, V.views, 9, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD,
+                  masters=W.views if master else None)
+    for i, n in enumerate(sizes):
+        args = ((w or p)[i], g[i], m[i], v[i], 9, LR, BETAS, EPS, WD)
+        want, tol = orc.adamw64(*args), orc.adamw_tolerance(*args)
+        _assert_close(M.views[i], want[1], tol[1], f"exp_avg {n}")
+        _assert_close(V.views[i], want[2], tol[2], f"exp_avg_sq {n}")
+        if master:
+            _assert_close(W.views[i], want[0], tol[0], f"master {n}")
+        _assert_close(P.views[i], want[0], tol[0] + _half_step(want[0], t) * (1 + 2.0 ** -20), f"parameter {n}")
+    assert all(x.intact() for x in (P, G, M, V)) and (W is None or W.intact())
+    # 8-bit moments
+    pairs = {k: [orc.quantize(x, kind) for x in y] for k, kind, y in (("m", "exp_avg", m), ("v", "exp_avg_sq", v))}
+    C = {k: _Guarded([c for c, _ in pairs[k]], torch.uint8, o) for k, o in (("m", mo), ("v", vo))}
+    S = {k: _Guarded([s for _, s in pairs[k]], torch.float32, o) for k, o in (("m", vo), ("v", mo))}
+    before = [x.cpu().clone() for x in (W or P).views]
+    mb.adamw8_step(P.views, G.views, C["m"].views, S["m"].views, C["v"].views, S["v"].views, 9, lr=LR, betas=BETAS, eps=EPS,
+                   weight_decay=WD, masters=W.views if master else None, seed=4)
+    for i, n in enumerate(sizes):
+        m0, v0 = orc.dequantize(*pairs["m"][i], "exp_avg"), orc.dequantize(*pairs["v"][i], "exp_avg_sq")
+        m1, v1 = orc.moments32(g[i], m0, v0, BETAS)
+        _check_codes(C["m"].views[i], S["m"].views[i], orc.quantize(m1, "exp_avg"), "exp_avg", f"exp_avg {n}")
+        _check_codes(C["v"].views[i], S["v"].views[i], orc.quantize(v1, "exp_avg_sq", orc.random_bits(n, 4, 9)), "exp_avg_sq",
+                     f"exp_avg_sq {n}")
+        args = (before[i], g[i], m0, v0, 9, LR, BETAS, EPS, WD)
+        want, tol = orc.adamw64(*args)[0], orc.adamw_tolerance(*args)[0]
+        if master:
+            _assert_close(W.views[i], want, tol, f"master {n}")
+            assert torch.equal(P.views[i], W.views[i].to(t))
+        else:
+            _assert_close(P.views[i], want, tol + _half_step(want, t), f"parameter {n}")
+    assert all(x.intact() for x in (P, G, C["m"], C["v"], S["m"], S["v"])) and (W is None or W.intact())
+    # conversions and clipping
+    X = _Guarded([x.abs() for x in v], t, po)
+    mb.quantize_state(X.views, "exp_avg_sq", codes=C["v"].views, scales=S["v"].views)
+    mb.dequantize_state(C["v"].views, S["v"].views, "exp_avg_sq", out=X.views)
+    for i, n in enumerate(sizes):
+        want = orc.quantize(v[i].abs().to(t), "exp_avg_sq")
+        _check_codes(C["v"].views[i], S["v"].views[i], want, "exp_avg_sq", f"quantized {n}")
+        assert torch.equal(X.views[i].cpu(), orc.dequantize(*want, "exp_avg_sq").to(t))
+    norm, factor = mb.grad_norm(G.views, 1e-3)
+    mb.clip_grad_norm_(G.views, 1e-3)
+    assert all(torch.equal(a.cpu(), (b.float() * factor.cpu()).to(t)) for a, b in zip(G.views, g))
+    assert all(x.intact() for x in (X, G, C["v"], S["v"]))
+
+
 def test_adamw8_from_zero_state_and_zero_gradients(mb):
     """New state is all zeros; a block without gradients stays zero and its parameters only decay."""
     p = [torch.randn(1000), torch.randn(512)]
