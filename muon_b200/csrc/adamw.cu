@@ -182,9 +182,11 @@ __device__ __forceinline__ float moved(float p, float m, float v, float decay, f
 }
 
 // The factor that every gradient is multiplied by. A factor that is not finite (the norm was not)
-// means: leave everything as it is.
+// means: leave everything as it is. Waits for the kernel before this one, which may have left the factor
+// (launch_after); nothing is read or written before.
 __device__ __forceinline__ bool read_factor(const float* grad_scale, float& f) {
-  f = grad_scale ? __ldg(grad_scale) : 1.f;
+  griddep_wait();
+  f = grad_scale ? *grad_scale : 1.f;
   return fabsf(f) <= 3.402823466e38f;
 }
 
@@ -324,13 +326,12 @@ __device__ __forceinline__ float warp_max(uint32_t bits) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, bits));
 }
 __device__ __forceinline__ uint32_t amax_bits(const float2 (&x)[4]) {
-  uint32_t b[8];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    b[2 * j] = __float_as_uint(x[j].x) & 0x7fffffffu;
-    b[2 * j + 1] = __float_as_uint(x[j].y) & 0x7fffffffu;
-  }
-  return __vimax3_u32(__vimax3_u32(b[0], b[1], b[2]), __vimax3_u32(b[3], b[4], b[5]), max(b[6], b[7]));
+  float m;
+  asm("{\n\tmax.NaN.abs.f32 %0, %1, %2, %3;\n\tmax.NaN.abs.f32 %0, %0, %4, %5;\n\tmax.NaN.abs.f32 %0, %0, %6, %7;\n\t"
+      "max.NaN.abs.f32 %0, %0, %8, %8;\n\t}"
+      : "=&f"(m)
+      : "f"(x[0].x), "f"(x[0].y), "f"(x[1].x), "f"(x[1].y), "f"(x[2].x), "f"(x[2].y), "f"(x[3].x), "f"(x[3].y));
+  return __float_as_uint(m);
 }
 // The same for values that have no sign bit (a sum of squares; an arithmetic NaN has none either).
 __device__ __forceinline__ uint32_t amax_bits_unsigned(const float2 (&x)[4]) {
@@ -892,6 +893,7 @@ template <int CAP>
 __global__ void __launch_bounds__(kThreads, kNormBlocksPerSm)
 norm_partial_kernel(const __grid_constant__ NormArgs<CAP> a) {
   __shared__ double warps[kWarps];
+  griddep_launch_dependents();
   double acc = 0.0;
   for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) acc += squares_of(a, chunk);
   acc = block_sum(acc, warps);
@@ -918,6 +920,8 @@ __device__ __forceinline__ float2 finish_norm(const double* partials, int n, flo
 __global__ void __launch_bounds__(kThreads)
 norm_finish_kernel(const double* partials, int n, float max_norm, float* out2) {
   __shared__ double warps[kWarps];
+  griddep_launch_dependents();
+  griddep_wait();
   const float2 r = finish_norm(partials, n, max_norm, warps);
   if (threadIdx.x == 0) {
     out2[0] = r.x;
@@ -983,6 +987,7 @@ norm_cluster_kernel(const __grid_constant__ NormArgs<CAP> a, float max_norm, flo
   __shared__ double warps[kWarps];
   __shared__ double mine;
   const cg::cluster_group cluster = cg::this_cluster();
+  griddep_launch_dependents();
   double acc = 0.0;
   for (int chunk = blockIdx.x; chunk < a.chunks; chunk += kClusterBlocks) acc += squares_of(a, chunk);
   acc = block_sum(acc, warps);
@@ -1041,6 +1046,29 @@ int common_head(std::initializer_list<ListStart> lists) {
   return head;
 }
 
+// Launches a kernel that waits for its predecessor on the stream by itself (griddep_wait): its launch, with
+// arguments of up to 32 KB, then runs beside the predecessor's end where that one allows it
+// (griddep_launch_dependents). A norm's two kernels and a step with its factor follow one another so: 63.4 ->
+// 59.6 us for norm and step of 150 packed float16 tensors. Not the clipping pass: its blocks, which share the
+// work out evenly, were placed unevenly as the norm's left (437 MB: 121 -> 129 us).
+template <typename... Params, typename... Args>
+int launch_after(void (*kernel)(Params...), int grid, size_t shared, cudaStream_t stream, bool dependent,
+                 const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent && dependent_launch_enabled() ? 1 : 0;
+  MB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  MB_CUDA_CHECK(cudaGetLastError());
+  return OK;
+}
+
 // Adds `chunks` to the running total of a launch; false when the launch must go out first.
 inline bool fits(int total, int64_t chunks) { return chunks <= (int64_t)INT32_MAX - total; }
 
@@ -1067,8 +1095,8 @@ int adamw32_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t s
       if (n > 0) {
         a.c.count = n;
         LaunchScope scope(K_ADAMW, elems * bytes, stream);
-        adamw32_kernel<P, G, MASTER, CAP><<<a.start[n], kThreads, 0, stream>>>(a);
-        MB_CUDA_CHECK(cudaGetLastError());
+        const int rc = launch_after(adamw32_kernel<P, G, MASTER, CAP>, a.start[n], 0, stream, c.grad_scale != nullptr, a);
+        if (rc != OK) return rc;
       }
       n = 0;
       elems = 0;
@@ -1125,8 +1153,8 @@ int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t st
       if (n > 0) {
         a.c.count = n;
         LaunchScope scope(K_ADAMW, elems * bytes, stream);
-        adamw8_kernel<P, G, MASTER, CAP><<<a.start[n], kThreads, kShared, stream>>>(a);
-        MB_CUDA_CHECK(cudaGetLastError());
+        rc = launch_after(adamw8_kernel<P, G, MASTER, CAP>, a.start[n], kShared, stream, c.grad_scale != nullptr, a);
+        if (rc != OK) return rc;
       }
       n = 0;
       elems = 0;
@@ -1370,9 +1398,7 @@ int clip_launch(void* const* tensors, const int64_t* numel, const int* dtypes, i
       });
   if (rc != OK || launched) return rc;
   LaunchScope scope(K_GRAD_NORM, 0.0, stream);  // nothing but empty tensors: the norm is 0
-  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, 0, (float)max_norm, out2);
-  MB_CUDA_CHECK(cudaGetLastError());
-  return OK;
+  return launch_after(norm_finish_kernel, 1, 0, stream, false, static_cast<const double*>(partials), 0, (float)max_norm, out2);
 }
 }  // namespace
 
@@ -1385,9 +1411,7 @@ int run_grad_norm(void* const* tensors, const int64_t* numel, const int* dtypes,
                         : norm_partials<kCapNorm>(tensors, numel, dtypes, count, partials, &n, stream);
   if (rc != OK) return rc;
   LaunchScope scope(K_GRAD_NORM, 8.0 * n, stream);
-  norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, n, (float)max_norm, out2);
-  MB_CUDA_CHECK(cudaGetLastError());
-  return OK;
+  return launch_after(norm_finish_kernel, 1, 0, stream, n > 0, static_cast<const double*>(partials), n, (float)max_norm, out2);
 }
 
 int run_clip(void* const* tensors, const int64_t* numel, const int* dtypes, int count, double max_norm,
