@@ -396,11 +396,11 @@ int muon_b200_quantize_state(void* const* src, void* const* codes, void* const* 
 int muon_b200_dequantize_state(void* const* codes, void* const* scales, void* const* dst, const int64_t* numel,
                                int count, int dtype, int kind, muon_b200_stream_t stream);
 
-/* Norm of all elements of `count` tensors (each with its own element type) and the factor that
- * brings it down to max_norm, both left on the device: out2[0] = norm, out2[1] = min(1, max_norm /
+/* Norm of all elements of `count` tensors (at most 65536, each with its own element type) and the
+ * factor that brings it down to max_norm, both left on the device: out2[0] = norm, out2[1] = min(1, max_norm /
  * (norm + 1e-6)), or NaN when the norm is not finite, which makes an AdamW call that reads it change
  * nothing. The squares of the whole range of float32 are added up without overflow. The order of the
- * additions depends on the sizes and the device only. scratch: 256-byte aligned, at least
+ * additions depends on sizes, alignment and the device only. scratch: 256-byte aligned, at least
  * muon_b200_grad_norm_scratch_bytes() bytes, contents irrelevant before and after; not shared with
  * a call that may run at the same time. */
 int64_t muon_b200_grad_norm_scratch_bytes(void);

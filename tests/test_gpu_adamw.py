@@ -55,15 +55,17 @@ def _half_step(x, dtype):
     return x.abs() * (info.eps / 2) + info.tiny * info.eps / 2
 
 
+# parameter type, master weights, gradient type
+_FORMS = [("fp32", False, "same")] + [(d, w, g) for d in ("bf16", "fp16") for w in (False, True) for g in ("same", "fp32")]
+
+
+@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])  # both sizes of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
-@pytest.mark.parametrize("grad", ["same", "fp32"])
-@pytest.mark.parametrize("master", [False, True], ids=["plain", "master"])
-@pytest.mark.parametrize("dtype", list(DTYPES))
-def test_adamw_step(mb, dtype, master, grad, offset):
+@pytest.mark.parametrize("dtype,master,grad", _FORMS, ids=["-".join((d, "master" if w else "plain", g)) for d, w, g in _FORMS])
+def test_adamw_step(mb, dtype, master, grad, offset, times):
     t = DTYPES[dtype]
-    if t == torch.float32 and (master or grad == "fp32"):
-        pytest.skip("float32 parameters: one form")
-    p, g, m, v = _inputs(SIZES, 1, t)
+    sizes = SIZES * times
+    p, g, m, v = _inputs(sizes, 1, t)
     if grad == "fp32":
         g = [x.float() * 1.001 for x in g]
     gen = torch.Generator().manual_seed(2)
@@ -75,7 +77,7 @@ def test_adamw_step(mb, dtype, master, grad, offset):
     factor = torch.tensor(0.37, device="cuda")
     mb.adamw_step(P, G, M, V, steps, lr=LR, betas=BETAS, eps=EPS, weight_decay=WD, masters=W, grad_scale=factor)
     f = float(torch.tensor(0.37))  # the factor as float32
-    for i, n in enumerate(SIZES):
+    for i, n in enumerate(sizes):
         args = ((w or p)[i], g[i], m[i], v[i], steps[i], LR, BETAS, EPS, WD, f)
         want = orc.adamw64(*args)
         tol = orc.adamw_tolerance(*args)
@@ -110,28 +112,27 @@ def _check_codes(got_codes, got_scales, want, kind, what):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} codes differ, first at {int(bad.nonzero()[0])}"
 
 
+@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])  # both sizes of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
-@pytest.mark.parametrize("master", [False, True], ids=["plain", "master"])
-@pytest.mark.parametrize("dtype", list(DTYPES))
-def test_adamw8_step(mb, dtype, master, offset):
+@pytest.mark.parametrize("dtype,master,grad", _FORMS, ids=["-".join((d, "master" if w else "plain", g)) for d, w, g in _FORMS])
+def test_adamw8_step(mb, dtype, master, grad, offset, times):
     """Two steps: every code and scale equal to the format's definition, parameters within the
     bounds of the float32 arithmetic."""
     t = DTYPES[dtype]
-    if t == torch.float32 and master:
-        pytest.skip("float32 parameters have no masters")
-    p, _, m, v = _inputs(SIZES, 3, t)
+    sizes = SIZES * times
+    p, _, m, v = _inputs(sizes, 3, t)
     host, dev = _state8(m, v, offset)
     P = _place(p, t, offset)
     w = [x.float() for x in p] if master else None
     W = _place(w, torch.float32, offset) if master else None
     seed = 0x12345678F
     for step in (41, 42):
-        g = _inputs(SIZES, 100 + step, t)[1]
-        G = _place(g, t, offset)
+        g = _inputs(sizes, 100 + step, t if grad == "same" else torch.float32)[1]
+        G = _place(g, g[0].dtype, offset)
         before = [x.cpu().clone() for x in (W or P)]
         mb.adamw8_step(P, G, dev["m"], dev["ms"], dev["v"], dev["vs"], step, lr=LR, betas=BETAS, eps=EPS,
                        weight_decay=WD, masters=W, seed=seed)
-        for i, n in enumerate(SIZES):
+        for i, n in enumerate(sizes):
             m0 = orc.dequantize(*host["m"][i], "exp_avg")
             v0 = orc.dequantize(*host["v"][i], "exp_avg_sq")
             m1, v1 = orc.moments32(g[i], m0, v0, BETAS)
@@ -445,20 +446,22 @@ def test_elements_past_32_bits(mb):
 
 
 # ------------------------------------------------------------------------------------ conversion
+@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["exp_avg", "exp_avg_sq"])
-def test_convert_state(mb, kind, dtype, offset):
+def test_convert_state(mb, kind, dtype, offset, times):
     t = DTYPES[dtype]
     gen = torch.Generator().manual_seed(14)
-    x = [(torch.randn(n, generator=gen) * torch.exp(2 * torch.randn(n, generator=gen))).to(t) for n in SIZES]
+    sizes = SIZES * times
+    x = [(torch.randn(n, generator=gen) * torch.exp(2 * torch.randn(n, generator=gen))).to(t) for n in sizes]
     if kind == "exp_avg_sq":
         x = [y.abs() for y in x]
     for y in x:
         y[:300:7] = 0
     X = _place(x, t, offset)
     codes, scales = mb.quantize_state(X, kind)
-    for i, n in enumerate(SIZES):
+    for i, n in enumerate(sizes):
         want = orc.quantize(x[i], kind)
         _check_codes(codes[i], scales[i], want, kind, f"{kind} {n}")
         assert codes[i].shape == x[i].shape and scales[i].numel() == -(-n // 256)
@@ -466,7 +469,7 @@ def test_convert_state(mb, kind, dtype, offset):
     for got, c, s in zip(mb.dequantize_state(C, S, kind, dtype=t), codes, scales):
         want = orc.dequantize(c.cpu(), s.cpu(), kind)
         assert got.dtype == t and torch.equal(got.cpu(), want.to(t))
-    out = _place([torch.zeros(n) for n in SIZES], torch.float32, offset)
+    out = _place([torch.zeros(n) for n in sizes], torch.float32, offset)
     assert mb.dequantize_state(C, S, kind, out=out) is out
     for got, y, s in zip(out, x, scales):  # half a code: 1/16 of the value, or half the smallest code
         y, s = y.double(), s.cpu().repeat_interleave(256)[:y.numel()].double()
