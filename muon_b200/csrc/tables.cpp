@@ -84,16 +84,17 @@ struct Lists {
         return false;
       }
       const at::Tensor& t = THPVariable_Unpack(o);
-      if (!t.is_cuda()) {
+      const at::Device where = t.device();
+      if (!where.is_cuda()) {
         PyErr_Format(PyExc_RuntimeError,
                      "muon_b200: every %s tensor of %s must live on a CUDA (sm_100) device, got device=%s; "
-                     "there is no CPU implementation", name, what, t.device().str().c_str());
+                     "there is no CPU implementation", name, what, where.str().c_str());
         return false;
       }
-      if (device < 0) device = t.get_device();
-      if (t.get_device() != device) {
+      if (device < 0) device = where.index();
+      if (where.index() != device) {
         PyErr_Format(PyExc_ValueError, "%s: %s tensors must all be on cuda:%lld, got %s", what, name,
-                     (long long)device, t.device().str().c_str());
+                     (long long)device, where.str().c_str());
         return false;
       }
       const int bit = type_bit(t.scalar_type());
@@ -104,7 +105,7 @@ struct Lists {
         return false;
       }
       found |= bit;
-      if (!t.has_storage()) {
+      if (!t.has_storage() || t.is_neg()) {  // (sparse ones, say; the negative of another tensor's memory)
         PyErr_Format(PyExc_ValueError, "%s: %s %zd has no memory of its own", what, name, i);
         return false;
       }

@@ -59,7 +59,7 @@ def _half_step(x, dtype):
 _FORMS = [("fp32", False, "same")] + [(d, w, g) for d in ("bf16", "fp16") for w in (False, True) for g in ("same", "fp32")]
 
 
-@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])  # both sizes of table
+@pytest.mark.parametrize("times", [1, 7, 18], ids=["few", "some", "many"])  # each size of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
 @pytest.mark.parametrize("dtype,master,grad", _FORMS, ids=["-".join((d, "master" if w else "plain", g)) for d, w, g in _FORMS])
 def test_adamw_step(mb, dtype, master, grad, offset, times):
@@ -112,7 +112,7 @@ def _check_codes(got_codes, got_scales, want, kind, what):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} codes differ, first at {int(bad.nonzero()[0])}"
 
 
-@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])  # both sizes of table
+@pytest.mark.parametrize("times", [1, 7, 18], ids=["few", "some", "many"])  # each size of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
 @pytest.mark.parametrize("dtype,master,grad", _FORMS, ids=["-".join((d, "master" if w else "plain", g)) for d, w, g in _FORMS])
 def test_adamw8_step(mb, dtype, master, grad, offset, times):
@@ -356,7 +356,7 @@ def _norm_error(n):
     return (4 + 1) * 2.0 ** -24
 
 
-@pytest.mark.parametrize("times", [1, 3, 9], ids=["few", "some", "many"])  # one launch, and both sizes of table
+@pytest.mark.parametrize("times", [1, 3, 9, 18], ids=["one", "few", "some", "many"])  # one launch, each size of table
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
 def test_grad_norm_and_clip(mb, offset, times):
     gen = torch.Generator().manual_seed(12)
@@ -446,7 +446,7 @@ def test_elements_past_32_bits(mb):
 
 
 # ------------------------------------------------------------------------------------ conversion
-@pytest.mark.parametrize("times", [1, 7], ids=["few", "many"])
+@pytest.mark.parametrize("times", [1, 7, 18], ids=["few", "some", "many"])
 @pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "odd"])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", ["exp_avg", "exp_avg_sq"])
@@ -533,6 +533,40 @@ def test_on_another_stream(mb):
         args = (p[i], g[i], m[i], v[i], 3, LR, BETAS, EPS, WD, f)
         _assert_close(P[i], orc.adamw64(*args)[0], orc.adamw_tolerance(*args)[0], "parameter")
         assert (back[i] - M[i]).abs().max() <= M[i].abs().max() / 16
+
+
+def test_two_streams_at_once(mb):
+    """Norm, clipping and both steps on two streams side by side: each as alone."""
+    def setup(seed):
+        p, g, m, v = _inputs([700001, 333, 90000], seed)
+        return dict(p=_place(p, torch.float32, 0), g=_place(g, torch.float32, 0), m=_place(m, torch.float32, 0),
+                    v=_place(v, torch.float32, 0), d=_state8(m, v, 0)[1])
+
+    def work(s):
+        norms = []
+        for step in range(3, 9):
+            norm, f = mb.grad_norm(s["g"], 0.7)
+            mb.adamw_step(s["p"], s["g"], s["m"], s["v"], step, grad_scale=f)
+            d = s["d"]
+            mb.adamw8_step(s["p"], s["g"], d["m"], d["ms"], d["v"], d["vs"], step, grad_scale=f, seed=step)
+            norms += [norm, mb.clip_grad_norm_(s["g"], 0.6)]
+        return norms
+
+    alone = [setup(k) for k in (50, 51)]
+    want = [work(s) for s in alone]
+    both = [setup(k) for k in (50, 51)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s, st in zip(both, streams):
+        with torch.cuda.stream(st):
+            got.append(work(s))
+    torch.cuda.synchronize()
+    for a, b, x, y in zip(alone, both, want, got):
+        assert all(torch.equal(i, j) for i, j in zip(x, y))
+        for key in ("p", "g", "m", "v"):
+            assert all(torch.equal(i, j) for i, j in zip(a[key], b[key])), key
+        for key in ("m", "ms", "v", "vs"):
+            assert all(torch.equal(i, j) for i, j in zip(a["d"][key], b["d"][key])), key
 
 
 def test_gradients_marked_ready_on_a_copy_stream(mb):
@@ -631,6 +665,8 @@ def test_refusals(mb):
         (lambda: mb.clip_grad_norm_([f()], -1.0), mb.MuonB200Error, "max_norm"),
         (lambda: mb.clip_grad_norm_([f()], float("nan")), mb.MuonB200Error, "max_norm"),
         (lambda: mb.grad_norm([f(dtype=torch.int32)]), ValueError, "int32"),
+        (lambda: mb.grad_norm([torch.view_as_complex(f(20).view(10, 2)).conj().imag]), ValueError, "no memory of its own"),
+        (lambda: mb.grad_norm([f().to_sparse()]), (ValueError, RuntimeError), "."),
     ]
     for k, (call, error, match) in enumerate(cases):
         with pytest.raises(error, match=match):
