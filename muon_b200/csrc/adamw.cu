@@ -601,7 +601,7 @@ constexpr int kShared8 = kWarps * kStages8 * Stage8<P, G, MASTER>::kBytes;
 // copied itself, so no barrier is needed and the loads in flight hold no registers. Scales are read and
 // written once per task, lane k's for block k.
 // 436M bf16 weights: 655 us, 6.7 TB/s (1592 with plain loads, 1039 with the next block's loads in
-// registers); under the power cap, at 1.58 GHz, 755 us: 42 instructions an element keep the ALU pipe busy.
+// registers); under the power cap, at 1.58 GHz, 755 us: 41 instructions an element keep the ALU pipe busy.
 // Lists that are not aligned go element by element (ragged_block8), at 3.1 to 4.1 TB/s.
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm8)
