@@ -1,0 +1,85 @@
+"""The AdamW operators and class, without a GPU: calls that lost state, counts or options."""
+import pytest
+import torch
+
+from test_adamw import _OracleBackend, _give_grads, _params
+
+
+@pytest.fixture
+def backend():
+    from muon_b200 import engine
+    prev = engine._set_backend_for_testing(_OracleBackend())
+    yield engine.get_backend()
+    engine._set_backend_for_testing(prev)
+
+
+def _assert_same_state(a, b):
+    assert set(a) == set(b)
+    for key, value in a.items():
+        if torch.is_tensor(value):
+            assert b[key].dtype == value.dtype and torch.equal(b[key], value) and b[key].data_ptr() != value.data_ptr(), key
+        else:
+            assert type(b[key]) is type(value) and b[key] == value, key
+
+
+# ------------------------------------------------------------------------------- consolidated checkpoints
+@pytest.mark.parametrize("bits", [32, 8])
+def test_consolidated_checkpoint_of_the_adamw_class(backend, bits, tmp_path):
+    import muon_b200 as mb
+    params = _params(1)
+    opt = mb.AdamW([dict(params=params[:2], lr=1e-2), dict(params=params[2:], master_weights=True)], state_bits=bits)
+    for k in range(3):
+        _give_grads(params, k)
+        opt.step()
+    torch.save(mb.consolidated_state_dict(opt), tmp_path / "state.pt")
+    copies = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    again = mb.AdamW([dict(params=copies[:2]), dict(params=copies[2:])], state_bits=40 - bits)
+    mb.load_consolidated_state_dict(again, torch.load(tmp_path / "state.pt"))
+    assert [g["lr"] for g in again.param_groups] == [1e-2, 1e-3] and again.param_groups[0]["state_bits"] == bits
+    for p, q in zip(params, copies):
+        assert opt.state[p]["step"] == 3
+        _assert_same_state(opt.state[p], again.state[q])
+    _give_grads(params, 9)
+    _give_grads(copies, 9)
+    opt.step()
+    again.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, copies))
+
+
+def test_consolidated_checkpoints_of_other_kinds_are_refused(backend):
+    """Muon state for an AdamW group or the reverse, an optimizer whose state is neither: refused, and what
+    the optimizer holds stays."""
+    import muon_b200 as mb
+    params = _params(2)[:1]
+    adamw, muon = mb.AdamW(params), mb.SingleDeviceMuon(params)
+    _give_grads(params, 1)
+    adamw.step()
+    muon.state[params[0]]["momentum_buffer"] = torch.ones(64, 80)
+    of_adamw, of_muon = mb.consolidated_state_dict(adamw), mb.consolidated_state_dict(muon)
+    for target, source in ((adamw, of_muon), (muon, of_adamw)):
+        with pytest.raises(ValueError, match="state of"):
+            mb.load_consolidated_state_dict(target, source)
+    assert adamw.state[params[0]]["step"] == 1 and (muon.state[params[0]]["momentum_buffer"] == 1).all()
+    other = torch.optim.AdamW(params)
+    other.step()
+    with pytest.raises(ValueError, match="exp_avg"):
+        mb.consolidated_state_dict(other)
+
+
+def test_consolidated_checkpoint_of_sharded_parameters_is_refused(backend, tmp_path):
+    """The state of a DTensor is that of this rank's rows: one rank's would be taken for all."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Shard
+    import muon_b200 as mb
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/pg", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        p = torch.nn.Parameter(DTensor.from_local(torch.randn(8, 4), mesh, [Shard(0)]))
+        p.grad = DTensor.from_local(torch.randn(8, 4), mesh, [Shard(0)])
+        opt = mb.AdamW([p])
+        opt.step()
+        with pytest.raises(ValueError, match="DTensor"):
+            mb.consolidated_state_dict(opt)
+    finally:
+        dist.destroy_process_group()
