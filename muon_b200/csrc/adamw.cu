@@ -371,7 +371,13 @@ __device__ __forceinline__ float sq_value(uint32_t word) {
   const uint32_t c = J < 3 ? word << (J < 3 ? 20 - 8 * J : 0) : word >> 4;
   return __uint_as_float((c & 0x0ff00000u) | 0x30000000u);
 }
-__device__ __forceinline__ int sq_cut(float x, uint32_t r) { return (int)(__float_as_uint(x) + r - 0x30000000u) >> 20; }
+// SIGNED: x may be -0 or negative, which is cut to the smallest code (with the sign bit among the others a
+// negative x close to zero would come out as the largest). A step's sums of squares have no sign.
+template <bool SIGNED>
+__device__ __forceinline__ int sq_cut(float x, uint32_t r) {
+  const uint32_t bits = SIGNED ? (uint32_t)max((int)__float_as_uint(x), 0) : __float_as_uint(x);
+  return (int)(bits + r - 0x30000000u) >> 20;
+}
 // Two integers clamped to 0..255 as bytes 0 and 1, bytes 2 and 3 from the low half of `high`.
 __device__ __forceinline__ uint32_t pack_bytes(int b1, int b0, uint32_t high) {
   uint32_t d;
@@ -400,7 +406,7 @@ __device__ __forceinline__ void decode8(uint2 w, float scale, float2 (&x)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[j] = mul2(x[j], both(scale));
 }
-template <int KIND>
+template <int KIND, bool SIGNED = false>
 __device__ __forceinline__ uint2 encode8(const float2 (&x)[4], float inv, const uint32_t (&r)[8]) {
   const float2 f = make_float2(inv, inv);
   float2 y[4];
@@ -412,8 +418,8 @@ __device__ __forceinline__ uint2 encode8(const float2 (&x)[4], float inv, const 
     uint32_t u[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      u[h] = pack_bytes(sq_cut(y[2 * h].y, r[4 * h + 1]), sq_cut(y[2 * h].x, r[4 * h]),
-                        pack_bytes(sq_cut(y[2 * h + 1].y, r[4 * h + 3]), sq_cut(y[2 * h + 1].x, r[4 * h + 2]), 0u));
+      u[h] = pack_bytes(sq_cut<SIGNED>(y[2 * h].y, r[4 * h + 1]), sq_cut<SIGNED>(y[2 * h].x, r[4 * h]),
+                        pack_bytes(sq_cut<SIGNED>(y[2 * h + 1].y, r[4 * h + 3]), sq_cut<SIGNED>(y[2 * h + 1].x, r[4 * h + 2]), 0u));
     return make_uint2(u[0], u[1]);
   }
 }
@@ -715,8 +721,10 @@ quantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
   const T* x = static_cast<const T*>(a.x[t]);
   uint8_t* codes = a.codes[t];
   const long long first = (long long)((int)blockIdx.x - a.start[t]) * kBlocksPerChunk + warp;
-  // half a code is added before the cut (an argument, because with the constant in its place the
-  // compiler's code saturated every value)
+  // Half a code is added before the cut. It is an argument because of the compiler (nvcc 12.9.86): with the
+  // constant 1 << 19 in its place the first element of every pair came out as 255 in this kernel, while the
+  // same expression in a kernel of its own is right for all 2^32 bit patterns, with either. The tests compare
+  // every code with the format's definition.
   const uint32_t r[8] = {a.half, a.half, a.half, a.half, a.half, a.half, a.half, a.half};
 #pragma unroll
   for (int k = 0; k < kBlocksPerWarp; ++k) {
@@ -739,7 +747,7 @@ quantize_kernel(const __grid_constant__ ConvertArgs<CAP> a) {
     }
     const float amax = warp_max(amax_bits(xj)), inv = block_factor<KIND>(amax);
     if (lane == 0) a.scales[t][b] = block_scale<KIND>(amax);
-    const uint2 c = encode8<KIND>(xj, inv, r);
+    const uint2 c = encode8<KIND, true>(xj, inv, r);
     if (vec) {
       __stcs(reinterpret_cast<uint2*>(codes + at), c);
     } else {
