@@ -42,6 +42,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
             parameters receive rounded copies.
         grad_scale: one float32 value on the device that every gradient is multiplied by (``grad_norm``
             returns one). When it is not finite nothing is changed.
+
+    No tensor that is written may share memory with another one of the call (a ValueError); gradients may with
+    each other.
     """
     get_backend().adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, weight_decay, betas, eps, masters,
                              grad_scale)

@@ -47,14 +47,15 @@ using Range = std::pair<uintptr_t, uintptr_t>;
 using Table = std::vector<void*>;
 enum Layout { kLikeFirst, kScales };  // sizes of a list: those of the first list, or one per block of its elements
 
-// The lists of one call. All tensors are on one device; what is written does not overlap.
+// The lists of one call. All tensors are on one device; what is written overlaps nothing else of the call (tensors
+// that are only read may share memory).
 struct Lists {
   const char* what;
   Py_ssize_t n = 0;
   int64_t device = -1;
   std::vector<int64_t> numel;
   std::vector<int> codes;  // element types of the first list
-  std::vector<Range> written;
+  std::vector<Range> written, read;
   Ref first;
 
   explicit Lists(const char* w) : what(w) {}
@@ -76,7 +77,7 @@ struct Lists {
     table.resize(n);
     found = 0;
     std::vector<Range> ranges;
-    if (writes) ranges.reserve(n);
+    ranges.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
       if (!THPVariable_Check(o)) {
@@ -134,15 +135,31 @@ struct Lists {
         return false;
       }
       table[i] = size == 0 ? nullptr : writes ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
-      if (writes && size > 0) {
+      if (size > 0) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(table[i]);
         ranges.emplace_back(at, at + size * t.element_size());
       }
     }
     if (is_first) first.p = fast.release();
-    if (writes && !merge(ranges)) {
+    if (!writes) {
+      read.insert(read.end(), ranges.begin(), ranges.end());
+    } else if (!merge(ranges)) {
       PyErr_Format(PyExc_ValueError, "%s: memory that is written (%s) appears twice in the call", what, name);
       return false;
+    }
+    return true;
+  }
+
+  // After the last list: false with a Python error set when something that is read lies in what is written.
+  bool reads_are_apart() {
+    if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+    size_t w = 0;  // first written range that ends behind the start of this read one
+    for (const Range& r : read) {
+      while (w < written.size() && written[w].second <= r.first) ++w;
+      if (w < written.size() && written[w].first < r.second) {
+        PyErr_Format(PyExc_ValueError, "%s: memory that is written overlaps memory that is read", what);
+        return false;
+      }
     }
     return true;
   }
@@ -233,7 +250,9 @@ PyObject* adamw(PyObject*, PyObject* args) {
       return PyErr_Format(PyExc_ValueError, "%s: grad_scale must be one float32 value on cuda:%lld", lists.what,
                           (long long)lists.device);
     factor = static_cast<const float*>(t->const_data_ptr());
+    lists.read.emplace_back(reinterpret_cast<uintptr_t>(factor), reinterpret_cast<uintptr_t>(factor + 1));
   }
+  if (!lists.reads_are_apart()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   void* const* wp = has_masters ? w.data() : nullptr;
@@ -263,7 +282,7 @@ PyObject* convert(PyObject*, PyObject* args) {
     return nullptr;
   if (lists.n == 0) return PyLong_FromLong(0);
   const int code = lists.one_type(types, "value");
-  if (code < 0) return nullptr;
+  if (code < 0 || !lists.reads_are_apart()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   const int n = static_cast<int>(lists.n);

@@ -38,3 +38,40 @@ def test_signed_zeros_of_second_moments(mb, dtype, offset):
         assert torch.equal(c.cpu(), want_c) and torch.equal(s.cpu(), want_s)
         assert (c.cpu()[torch.signbit(y)] == 0).all()
     assert (codes[4] == 0).all() and (scales[4] == 0).all()
+
+
+# ------------------------------------------------------------------------------------ memory
+def test_memory_that_is_read_and_written_is_refused(mb):
+    """A block would read what another one has written already. Each call is refused before a launch and leaves
+    the memory as it was; lists that lie close together in one buffer, or share what they only read, are not."""
+    f = lambda n=600, **k: torch.ones(n, device="cuda", **k)  # noqa: E731
+    u = lambda n=600: f(n, dtype=torch.uint8)  # noqa: E731
+    buf = f(1200)
+    codes = u(4800)
+    lie = codes.view(torch.float32)  # 1200 floats in the same memory
+    cases = [
+        lambda: mb.adamw_step([buf[:600]], [buf[300:900]], [f()], [f()], 1),
+        lambda: mb.adamw_step([buf[:600]], [buf[:600]], [f()], [f()], 1),
+        lambda: mb.adamw_step([f()], [buf[:600]], [buf[599:1199]], [f()], 1),
+        lambda: mb.adamw_step([f(), f()], [f(), buf[:600]], [f(), f()], [buf[500:1100], f()], 1),
+        lambda: mb.adamw_step([buf[:600]], [f()], [f()], [f()], 1, grad_scale=buf[599]),
+        lambda: mb.adamw_step([f(dtype=torch.bfloat16)], [buf[:600]], [f()], [f()], 1, masters=[buf[1:601]]),
+        lambda: mb.adamw8_step([f()], [lie[:600]], [codes[:600]], [f(3)], [u()], [f(3)], 1),
+        lambda: mb.adamw8_step([f()], [buf[:600]], [u()], [buf[598:601]], [u()], [f(3)], 1),
+        lambda: mb.quantize_state([lie[:600]], "exp_avg", codes=[codes[2399:2999]]),
+        lambda: mb.quantize_state([buf[:600]], "exp_avg", scales=[buf[597:600]]),
+        lambda: mb.dequantize_state([codes[:600]], [f(3)], "exp_avg", out=[lie[:600]]),
+        lambda: mb.dequantize_state([u()], [buf[600:603]], "exp_avg", out=[buf[1:601]]),
+    ]
+    for k, call in enumerate(cases):
+        with pytest.raises(ValueError, match="overlaps memory that is read"):
+            call()
+            pytest.fail(f"case {k} was accepted")
+    assert (buf == 1).all() and (codes == 1).all()
+    buf = f(2404)
+    mb.adamw_step([buf[:600]], [buf[600:1200]], [buf[1200:1800]], [buf[1800:2400]], 1, grad_scale=buf[2400])
+    assert (buf[600:1200] == 1).all() and (buf[:600] != 1).all() and buf[2400] == 1
+    g = f()
+    mb.adamw_step([f(), f()], [g, g], [f(), f()], [f(), f()], 1)
+    codes, scales = mb.quantize_state([g, g[:300]], "exp_avg")
+    mb.dequantize_state([codes[0], codes[0][:256]], [scales[0], scales[0][:1]], "exp_avg")
