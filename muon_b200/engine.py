@@ -69,7 +69,8 @@ def mark_grad_ready(tensor: Tensor, event: "torch.cuda.Event | None" = None) -> 
     makes the first kernel that reads the gradient wait for the event, launch group by launch
     group, so Newton-Schulz of the gradients that arrived first runs while later ones are still
     in flight. Gradients without a mark are assumed ready in the order of step()'s own stream,
-    which is the reference's behaviour. A mark is consumed by the step that uses it."""
+    which is the reference's behaviour. A mark is consumed by the step that uses it; a norm taken before waits
+    for it and leaves it, and clipping moves it behind the scaled values."""
     if isinstance(tensor, torch.nn.Parameter):
         if tensor.grad is None:
             raise ValueError("mark_grad_ready: the parameter has no gradient yet; allocate p.grad (or pass "
@@ -84,14 +85,15 @@ def mark_grad_ready(tensor: Tensor, event: "torch.cuda.Event | None" = None) -> 
     _grad_ready[g.data_ptr()] = event
 
 
-def _wait_grads(stream, grads: Sequence[Tensor]) -> None:
-    """Make `stream` wait for the readiness events of `grads` (those that have one)."""
+def _wait_grads(stream, grads: Sequence[Tensor], keep: bool = False) -> list[int]:
+    """Make `stream` wait for the readiness events of `grads` (those that have one), and drop the marks
+    unless they are kept. Returns the marked addresses."""
     if not _grad_ready:
-        return
-    for g in grads:
-        ev = _grad_ready.pop(g.data_ptr(), None)
-        if ev is not None:
-            stream.wait_event(ev)
+        return []
+    marked = [at for at in dict.fromkeys(g.data_ptr() for g in grads) if at in _grad_ready]
+    for at in marked:
+        stream.wait_event(_grad_ready[at] if keep else _grad_ready.pop(at))
+    return marked
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -579,10 +581,16 @@ class CudaBackend:
     def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> tuple[Tensor, Tensor]:
         """(norm, factor) of all `tensors` together, on their device; with `clip` the tensors are
         multiplied by the factor."""
+        marked = []
         if _grad_ready:
-            _wait_grads(torch.cuda.current_stream(tensors[0].device), tensors)
+            stream = torch.cuda.current_stream(tensors[0].device)
+            marked = _wait_grads(stream, tensors, keep=True)  # the step that follows may be on another stream
         rc, norm, factor = _tables.grad_norm(tensors, max_norm, clip, self._norm_scratch)
         check(rc)
+        if clip and marked:
+            scaled = torch.cuda.Event()
+            scaled.record(stream)
+            _grad_ready.update(dict.fromkeys(marked, scaled))
         self.launch_groups += 1
         return norm, factor
 

@@ -83,3 +83,71 @@ def test_consolidated_checkpoint_of_sharded_parameters_is_refused(backend, tmp_p
             mb.consolidated_state_dict(opt)
     finally:
         dist.destroy_process_group()
+
+
+# ------------------------------------------------------------------------------- marked gradients
+class _Stream:
+    """Stand-in for a CUDA stream: the events it was made to wait for, and what ran on it, in order."""
+
+    def __init__(self):
+        self.log = []
+
+    def wait_event(self, event):
+        self.log.append(event)
+
+
+class _Event:
+    def __init__(self):
+        self.after = None
+
+    def record(self, stream):
+        self.after = list(stream.log)
+
+
+@pytest.fixture
+def streams(monkeypatch):
+    """The current stream as a stand-in, and the marks; `streams.now` may be set to another stream."""
+    from muon_b200 import engine
+
+    class Streams:
+        now = _Stream()
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Streams.now)
+    monkeypatch.setattr(torch.cuda, "Event", _Event)
+    monkeypatch.setattr(engine, "_grad_ready", {})
+    return Streams
+
+
+@pytest.mark.parametrize("clip", [False, True])
+def test_a_norm_leaves_the_marks_to_the_step(streams, monkeypatch, clip):
+    """A norm on one stream waits for marked gradients, and so does the step on another stream that follows it;
+    after clipping the step waits for the clipped values."""
+    from muon_b200 import engine
+    calls = engine.CudaBackend()
+
+    class Tables:
+        @staticmethod
+        def grad_norm(tensors, max_norm, clip, scratch):
+            streams.now.log.append("norm")
+            return 0, torch.ones(()), torch.ones(())
+
+        @staticmethod
+        def adamw(*args):
+            streams.now.log.append("step")
+            return 0
+
+    monkeypatch.setattr(engine, "_tables", Tables)
+    a, b = torch.zeros(4), torch.zeros(4)
+    arrived = _Event()
+    engine._grad_ready[a.data_ptr()] = arrived
+    first = streams.now
+    calls.grad_norm([a, b], 1.0, clip)
+    assert first.log == [arrived, "norm"]
+    streams.now = second = _Stream()
+    calls.adamw_step([a, b], [a, b], [a, b], [a, b], 1, 1e-3, 0.0, (0.9, 0.999), 1e-8)
+    assert len(second.log) == 2 and second.log[1] == "step"
+    if clip:
+        assert second.log[0].after == [arrived, "norm"]  # an event behind the clipping
+    else:
+        assert second.log[0] is arrived
+    assert not engine._grad_ready

@@ -75,3 +75,33 @@ def test_memory_that_is_read_and_written_is_refused(mb):
     mb.adamw_step([f(), f()], [g, g], [f(), f()], [f(), f()], 1)
     codes, scales = mb.quantize_state([g, g[:300]], "exp_avg")
     mb.dequantize_state([codes[0], codes[0][:256]], [scales[0], scales[0][:1]], "exp_avg")
+
+
+# ------------------------------------------------------------------------------------ marked gradients
+@pytest.mark.parametrize("clip", [False, True])
+def test_norm_and_step_of_marked_gradients_on_two_streams(mb, clip):
+    """Gradients that arrive on a copy stream, their norm on a second stream, the step on a third: the marks alone
+    order them."""
+    n = 1 << 20
+    gen = torch.Generator().manual_seed(31)
+    p, g = torch.randn(n, generator=gen) * 0.02, (torch.randn(n, generator=gen) * 1e-3).pin_memory()
+    P, G = _place([p], torch.float32, 0), [torch.zeros(n, device="cuda")]
+    M, V = ([torch.zeros(n, device="cuda")] for _ in range(2))
+    copies, norms, steps = (torch.cuda.Stream() for _ in range(3))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(copies):
+        torch.cuda._sleep(20_000_000)
+        G[0].copy_(g, non_blocking=True)
+        mb.mark_grad_ready(G[0])
+    with torch.cuda.stream(norms):
+        norm = mb.clip_grad_norm_(G, 0.5) if clip else mb.grad_norm(G, 0.5)[0]
+    with torch.cuda.stream(steps):
+        mb.adamw_step(P, G, M, V, 1, weight_decay=0.0)
+    torch.cuda.synchronize()
+    want_norm = float(g.double().norm())
+    assert abs(float(norm) - want_norm) <= 5 * 2.0 ** -24 * want_norm
+    factor = min(1.0, 0.5 / (want_norm + 1e-6)) if clip else 1.0
+    want = 0.1 * factor * g.double()  # roundings: norm 5, sum and quotient 2, the product, constant and product of the moment 2
+    assert ((M[0].cpu().double() - want).abs() <= 10.5 * 2.0 ** -24 * want.abs() + 1e-44).all()
+    from muon_b200 import engine
+    assert not engine._grad_ready
