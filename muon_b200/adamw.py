@@ -17,12 +17,7 @@ from torch import Tensor
 
 from ._lib import STATE_BLOCK
 from ._tables import gradients
-from .engine import _STATE_KINDS, _wait_grads, get_backend
-
-try:
-    from torch.distributed.tensor import DTensor
-except ImportError:  # pragma: no cover - torch without DTensor
-    DTensor = None
+from .engine import _STATE_KINDS, get_backend, local_part, wait_for_mark
 
 
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
@@ -166,8 +161,7 @@ def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, fl
     kinds: "OrderedDict[tuple, list]" = OrderedDict()
     for p, g, state in entries:
         if g.stride() != p.stride():  # a gradient in another order of dimensions than its parameter
-            if g.is_cuda:
-                _wait_grads(torch.cuda.current_stream(g.device), [g])
+            wait_for_mark(g)
             g = torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
         kinds.setdefault((p.dtype, g.dtype, p.device, state["moment_bits"], "master" in state), []).append((p, g, state))
     for (_, _, _, bits, master), members in kinds.items():
@@ -233,12 +227,7 @@ class KeepsMomentTypes:
         for i, p in zip(ids, (p for group in self.param_groups for p in group["params"])):
             saved = state_dict["state"].get(i, {})
             if "moment_bits" in saved:
-                self.state[p].update(restore_moments(_local(p), saved))
-
-
-def _local(t: Tensor) -> Tensor:
-    """This rank's part of a DTensor, or the tensor itself."""
-    return t.to_local() if DTensor is not None and isinstance(t, DTensor) else t
+                self.state[p].update(restore_moments(local_part(p), saved))
 
 
 class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
@@ -289,12 +278,13 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
         for group in self.param_groups:
             entries = []
             for p in group["params"]:
-                g, local = p.grad, _local(p)
+                g, local = p.grad, local_part(p)
                 if g is None:
                     continue
                 if local is not p:
                     sharded = True
                     if g.placements != p.placements:  # one that is not reduced yet, say
+                        wait_for_mark(g)
                         g = g.redistribute(placements=p.placements)
                     g = g.to_local()
                 entries.append((local, g, self.state[p]))
@@ -328,4 +318,4 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
         for group in self.param_groups:
             group["state_bits"] = bits
             convert_moments([self.state[p] for p in group["params"] if len(self.state.get(p, {})) > 0
-                             and (bits == 32 or _local(p).numel() >= group["min_8bit_numel"])], bits)
+                             and (bits == 32 or local_part(p).numel() >= group["min_8bit_numel"])], bits)

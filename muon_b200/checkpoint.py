@@ -13,7 +13,8 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
-from .adamw import AdamW, DTensor, restore_moments
+from .adamw import AdamW, restore_moments
+from .engine import DTensor
 from .ownership import owned_indices
 
 FORMAT = "muon_b200.consolidated.v1"

@@ -22,6 +22,11 @@ from . import _lib, _tables
 from ._lib import (BF16, EXP_AVG, EXP_AVG_SQ, F16, F32, F64, NS_AOL4, NS_AOL4_FP8, NS_CLASSIC5, NS_HAVE_SUMSQ,
                    check, i64_array, lib, ptr_array)
 
+try:
+    from torch.distributed.tensor import DTensor
+except ImportError:  # pragma: no cover - torch without DTensor
+    DTensor = None
+
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 # element types the cast at the entry of Newton-Schulz accepts (muon.py:760 takes any float dtype)
 _NS_INPUT_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.float64: F64}
@@ -55,6 +60,11 @@ def get_ns_mode() -> tuple[str, int]:
     return _ns_mode, _ns_steps
 
 
+def local_part(t: Tensor) -> Tensor:
+    """This rank's part of a DTensor, or the tensor itself."""
+    return t.to_local() if DTensor is not None and isinstance(t, DTensor) else t
+
+
 # Gradients that are produced on another stream than the one step() runs on (copied in from
 # host memory, reduced by a communication stream, written by a backward stream): the event that
 # completes when the gradient holds its value, keyed by the gradient's address.
@@ -75,9 +85,8 @@ def mark_grad_ready(tensor: Tensor, event: "torch.cuda.Event | None" = None) -> 
         if tensor.grad is None:
             raise ValueError("mark_grad_ready: the parameter has no gradient yet; allocate p.grad (or pass "
                              "the gradient tensor itself) before marking it")
-        g = tensor.grad
-    else:
-        g = tensor
+        tensor = tensor.grad
+    g = local_part(tensor)
     _require_cuda(g, "gradient")
     if event is None:
         event = torch.cuda.Event()
@@ -94,6 +103,14 @@ def _wait_grads(stream, grads: Sequence[Tensor], keep: bool = False) -> list[int
     for at in marked:
         stream.wait_event(_grad_ready[at] if keep else _grad_ready.pop(at))
     return marked
+
+
+def wait_for_mark(grad: Tensor) -> None:
+    """Make the current stream wait for a gradient that is about to be copied there."""
+    if _grad_ready:
+        grad = local_part(grad)
+        if grad.data_ptr() in _grad_ready:
+            _wait_grads(torch.cuda.current_stream(grad.device), [grad])
 
 
 def _stream_ptr(device: torch.device) -> int:

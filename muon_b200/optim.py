@@ -19,7 +19,7 @@ import torch
 import torch.distributed as dist
 
 from .adamw import _MIN_8BIT_NUMEL, KeepsMomentTypes, get_adam_moments, moments_step, new_moments
-from .engine import get_backend, plan_launches, view_2d
+from .engine import get_backend, plan_launches, view_2d, wait_for_mark
 from .exchange import get_peer_push
 from .ownership import get_ownership, owners
 
@@ -30,6 +30,7 @@ def _ensure_grad_and_state(optimizer, p) -> None:
     if p.grad is None:
         p.grad = torch.zeros_like(p)
     elif not p.grad.is_contiguous():
+        wait_for_mark(p.grad)
         p.grad = p.grad.contiguous()
     state = optimizer.state[p]
     if len(state) == 0:
@@ -70,6 +71,7 @@ def _adam_update_params(optimizer, group) -> None:
         if p.grad is None:
             p.grad = torch.zeros_like(p)
         elif not p.grad.is_contiguous():
+            wait_for_mark(p.grad)
             p.grad = p.grad.contiguous()
         state = optimizer.state[p]
         if len(state) == 0:

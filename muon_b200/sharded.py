@@ -31,7 +31,7 @@ from collections import OrderedDict
 import torch
 import torch.distributed as dist
 
-from .engine import get_backend, view_2d
+from .engine import get_backend, view_2d, wait_for_mark
 
 try:  # DTensor moved between releases; the class is only needed for isinstance checks
     from torch.distributed.tensor import DTensor
@@ -172,6 +172,7 @@ class _Unit:
         for slot, j in enumerate(self.order):
             g = self.plist[j].grad
             if g is not None and self.mine_rows:
+                wait_for_mark(g)
                 send[slot, :self.mine_rows].copy_(_local(g).reshape(self.mine_rows, cols))
         self.recv = torch.empty(world, self.n_mine, chunk, cols, dtype=dtype, device=dev)
         self.grad_work = dist.all_to_all_single(

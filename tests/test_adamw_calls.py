@@ -151,3 +151,81 @@ def test_a_norm_leaves_the_marks_to_the_step(streams, monkeypatch, clip):
     else:
         assert second.log[0] is arrived
     assert not engine._grad_ready
+
+
+class _Arrival(_Event):
+    """A gradient in flight: its values are there once a stream has waited for them."""
+
+    def __init__(self, gradient, values):
+        super().__init__()
+        self.gradient, self.values = gradient, values
+
+
+@pytest.fixture
+def in_flight(streams, monkeypatch):
+    """in_flight(gradient) makes it NaN until a wait for its mark brings its values."""
+    from muon_b200 import engine
+
+    def put(gradient):
+        engine._grad_ready[gradient.data_ptr()] = _Arrival(gradient, gradient.clone())
+        gradient.fill_(float("nan"))
+
+    monkeypatch.setattr(_Stream, "wait_event", lambda self, event: event.gradient.copy_(event.values))
+    yield put
+    assert not engine._grad_ready
+
+
+def test_copies_of_gradients_wait_for_their_marks(in_flight, backend):
+    """A gradient in another order of dimensions is copied before the kernels read it."""
+    import muon_b200 as mb
+    gen = torch.Generator().manual_seed(5)
+    grad = lambda: torch.randn(80, 64, generator=gen).t()  # noqa: E731
+    p = torch.nn.Parameter(torch.zeros(64, 80))
+    seen = []
+    backend.adam_step = lambda ps, gs, *rest: seen.extend(g.clone() for g in gs)
+    backend.muon_step = lambda ps, gs, *rest, **more: seen.extend(g.clone() for g in gs)
+    backend.adamw_step = lambda ps, gs, *rest: seen.extend(g.clone() for g in gs)
+    optimizers = [mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=False)]),
+                  mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=True)]), mb.SingleDeviceMuon([p]), mb.AdamW([p])]
+    for opt in optimizers:
+        p.grad = grad()
+        want = p.grad.clone()
+        in_flight(p.grad)
+        opt.step()
+        assert torch.equal(seen.pop(), want), type(opt).__name__
+
+
+def test_sharded_gradients_wait_for_their_marks(in_flight, backend, monkeypatch, tmp_path):
+    """Gradients that are DTensors are marked by the memory of their local part, and redistributed or sent off
+    after it is there."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Partial, Shard
+    import muon_b200 as mb
+    from muon_b200 import engine
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/pg", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        gen = torch.Generator().manual_seed(6)
+        g = torch.randn(8, 4, generator=gen)
+        p = torch.nn.Parameter(DTensor.from_local(torch.zeros(8, 4), mesh, [Shard(0)]))
+        seen = []
+        backend.adamw_step = lambda ps, gs, *rest: seen.extend(g.clone() for g in gs)
+        for placement in (Partial(), Shard(0)):
+            p.grad = DTensor.from_local(g.clone(), mesh, [placement])
+            if isinstance(placement, Partial):  # (a whole one is waited for by the call itself)
+                in_flight(p.grad.to_local())
+            mb.AdamW([p]).step()
+            assert torch.equal(seen.pop(), g)
+        backend.muon_orthogonalize = lambda grads, *rest: seen.extend(g.clone() for g in grads)
+        backend.apply_update = lambda *args: None
+        in_flight(p.grad.to_local())
+        mb.ShardedMuon([p]).step()
+        assert torch.equal(seen.pop(), g)
+        monkeypatch.setattr(engine, "_require_cuda", lambda *args: None)
+        for x in (p, p.grad):
+            mb.mark_grad_ready(x)
+            assert list(engine._grad_ready) == [p.grad.to_local().data_ptr()]
+            engine._grad_ready.clear()
+    finally:
+        dist.destroy_process_group()
