@@ -257,6 +257,14 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, min_8bit_numel=min_8bit_numel, seed=seed))
 
+    def __getstate__(self):  # (torch's holds defaults, state and groups only)
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "grad_norm": self.grad_norm}
+
+    def __setstate__(self, state):  # (torch's load_state_dict passes state and groups only)
+        super().__setstate__(state)
+        self.__dict__.setdefault("max_grad_norm", None)
+        self.__dict__.setdefault("grad_norm", None)
+
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
         group = self.param_groups[-1]

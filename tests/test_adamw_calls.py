@@ -229,3 +229,28 @@ def test_sharded_gradients_wait_for_their_marks(in_flight, backend, monkeypatch,
             engine._grad_ready.clear()
     finally:
         dist.destroy_process_group()
+
+
+# ------------------------------------------------------------------------------- copies of an optimizer
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+@pytest.mark.parametrize("max_norm", [None, 0.05])
+def test_a_copied_optimizer_steps_as_the_original(backend, how, max_norm):
+    import copy
+    import pickle
+    import muon_b200 as mb
+    params = _params(3)
+    opt = mb.AdamW(params, lr=1e-2, state_bits=8, max_grad_norm=max_norm)
+    _give_grads(params, 1)
+    opt.step()
+    again = copy.deepcopy(opt) if how == "deepcopy" else pickle.loads(pickle.dumps(opt))
+    copies = again.param_groups[0]["params"]
+    assert again.max_grad_norm == max_norm and (max_norm is None) == (again.grad_norm is None)
+    _give_grads(params, 2)
+    _give_grads(copies, 2)
+    opt.step()
+    again.step()
+    for p, q in zip(params, copies):
+        assert p is not q and torch.equal(p, q)
+        _assert_same_state(opt.state[p], again.state[q])
+    again.load_state_dict(opt.state_dict())
+    assert again.max_grad_norm == max_norm
