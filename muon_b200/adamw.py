@@ -151,7 +151,11 @@ def new_moments(state: dict, p: Tensor, bits: int, master: bool = False) -> None
             state[key] = torch.zeros_like(p, dtype=torch.uint8 if bits == 8 else torch.float32,
                                           memory_format=torch.preserve_format)
     if master:
-        state["master"] = p.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
+        state["master"] = _master_of(p)
+
+
+def _master_of(p: Tensor) -> Tensor:
+    return p.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
 
 
 def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
@@ -230,6 +234,39 @@ class KeepsMomentTypes:
                 self.state[p].update(restore_moments(local_part(p), saved))
 
 
+# what a group of another Adam holds and AdamW has no use for
+_FOREIGN_KEYS = {"amsgrad", "maximize", "foreach", "capturable", "differentiable", "fused", "decoupled_weight_decay", "use_muon"}
+
+
+def _adopted(state_dict: dict, param_groups: list[dict]) -> dict:
+    """The state dictionary of another Adam with decoupled decay as one of ``AdamW`` with float32 moments."""
+    groups, states = [], {}
+    for saved, mine in zip(state_dict["param_groups"], param_groups):
+        missing = {"lr", "betas", "eps", "weight_decay"} - set(saved)
+        if missing:
+            raise ValueError(f"not the state of an AdamW: a group without {sorted(missing)}")
+        for key in ("amsgrad", "maximize"):
+            if saved.get(key):
+                raise ValueError(f"AdamW does not take over a run with {key}")
+        if not saved.get("decoupled_weight_decay", True) and saved["weight_decay"] != 0:
+            raise ValueError("AdamW does not take over a run whose weight decay is not decoupled (torch.optim.Adam)")
+        groups.append({**{k: v for k, v in mine.items() if k != "params"},
+                       **{k: v for k, v in saved.items() if k not in _FOREIGN_KEYS}})
+        for i in saved["params"]:
+            if i in state_dict["state"]:
+                states[i] = _adopted_state(state_dict["state"][i])
+    return {**state_dict, "param_groups": groups + list(state_dict["param_groups"][len(groups):]), "state": states}
+
+
+def _adopted_state(saved: dict) -> dict:
+    if not saved or "moment_bits" in saved:
+        return saved
+    if set(saved) != {"step", "exp_avg", "exp_avg_sq"}:
+        raise ValueError(f"not the state of an AdamW: {sorted(saved)}")
+    return {"step": int(saved["step"]), "moment_bits": 32,
+            **{key: local_part(saved[key]).detach().to(torch.float32) for key in ("exp_avg", "exp_avg_sq")}}
+
+
 class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with one launch for all parameters of a type.
 
@@ -264,6 +301,24 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
         super().__setstate__(state)
         self.__dict__.setdefault("max_grad_norm", None)
         self.__dict__.setdefault("grad_norm", None)
+
+    def load_state_dict(self, state_dict):
+        """State of this class is loaded as it was saved. That of ``torch.optim.AdamW`` (or of an Adam group of
+        ``MuonWithAuxAdam``) is turned into this optimizer's: hyper-parameters from the dictionary,
+        ``state_bits``, ``master_weights`` and ``seed`` from here. What has another meaning (AMSGrad, maximizing, a
+        decay that is not decoupled, another optimizer's state) is refused."""
+        own = all("state_bits" in group for group in state_dict["param_groups"])
+        super().load_state_dict(state_dict if own else _adopted(state_dict, self.param_groups))
+        if own:
+            return
+        for group in self.param_groups:
+            held = [(p, self.state[p]) for p in group["params"] if self.state.get(p)]
+            for p, state in held:
+                local = local_part(p)
+                if group["master_weights"] and local.dtype != torch.float32 and "master" not in state:
+                    state["master"] = _master_of(local)
+            if group["state_bits"] == 8:
+                convert_moments([state for p, state in held if local_part(p).numel() >= group["min_8bit_numel"]], 8)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)

@@ -254,3 +254,124 @@ def test_a_copied_optimizer_steps_as_the_original(backend, how, max_norm):
         _assert_same_state(opt.state[p], again.state[q])
     again.load_state_dict(opt.state_dict())
     assert again.max_grad_norm == max_norm
+
+
+# ------------------------------------------------------------------------------- state of other optimizers
+def _two_runs(seed, kinds=(torch.float32, torch.float32)):
+    gen = torch.Generator().manual_seed(seed)
+    ps = [torch.nn.Parameter((torch.randn(s, generator=gen) * 0.1).to(k)) for s, k in zip(((70, 80), (5,)), kinds)]
+    return ps, [torch.nn.Parameter(p.detach().clone()) for p in ps]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_run_of_torch_adamw_goes_on(backend, bits):
+    """Moments, step numbers and the hyper-parameters of torch.optim.AdamW are taken over, into this optimizer's
+    kind of state. The stand-in computes in 64 bits, torch in 32; moments in 8 bits are half a code off."""
+    import muon_b200 as mb
+    theirs, ours = _two_runs(1)
+    run = torch.optim.AdamW([dict(params=theirs[:1], lr=1e-2), dict(params=theirs[1:])], lr=2e-3, betas=(0.8, 0.9),
+                            eps=1e-7, weight_decay=0.1)
+    for k in range(3):
+        _give_grads(theirs, k)
+        run.step()
+    for p, q in zip(theirs, ours):
+        q.data.copy_(p)
+    opt = mb.AdamW([dict(params=ours[:1], seed=4), dict(params=ours[1:])], state_bits=bits)
+    opt.load_state_dict(run.state_dict())
+    assert [(g["lr"], g["betas"], g["eps"], g["weight_decay"], g["state_bits"], g["seed"]) for g in opt.param_groups] == [
+        (1e-2, (0.8, 0.9), 1e-7, 0.1, bits, 4), (2e-3, (0.8, 0.9), 1e-7, 0.1, bits, 0)]
+    assert set(opt.param_groups[0]) == set(mb.AdamW([ours[0]]).param_groups[0])
+    assert [(opt.state[p]["step"], opt.state[p]["moment_bits"]) for p in ours] == [(3, bits), (3, 32)]
+    if bits == 32:
+        for p, q in zip(theirs, ours):
+            for key in ("exp_avg", "exp_avg_sq"):
+                assert torch.equal(run.state[p][key], opt.state[q][key])
+    _give_grads(theirs, 9)
+    _give_grads(ours, 9)
+    run.step()
+    opt.step()
+    for p, q in zip(theirs, ours):
+        # Half a code is 1/16 of either moment. With these betas |m| <= 1.18 sqrt(v) (Cauchy-Schwarz), at step 4 an
+        # update is at most 1.17 lr and the codes are worth 0.062 (m) + 0.038 (v) of lr
+        assert torch.allclose(p, q, rtol=1e-6, atol=1e-7 if bits == 32 or q.numel() == 5 else 1.2e-3)
+
+
+def test_torch_state_of_16_bit_parameters_becomes_float32(backend):
+    import muon_b200 as mb
+    theirs, ours = _two_runs(2, (torch.bfloat16, torch.float16))
+    run = torch.optim.AdamW(theirs)
+    _give_grads(theirs, 1)
+    run.step()
+    opt = mb.AdamW(ours, master_weights=True)
+    opt.load_state_dict(run.state_dict())
+    for p, q in zip(theirs, ours):
+        s = opt.state[q]
+        assert s["exp_avg"].dtype == s["exp_avg_sq"].dtype == s["master"].dtype == torch.float32
+        assert torch.equal(s["exp_avg"], run.state[p]["exp_avg"].float()) and torch.equal(s["master"], q.float())
+    _give_grads(ours, 2)
+    opt.step()
+
+
+def test_adam_groups_of_other_classes_are_taken_over(backend):
+    import muon_b200 as mb
+    ours = _params(4)[:2]
+    try:
+        for moments in ("param", "fp32", "8bit"):
+            mb.set_adam_moments(moments)
+            run = mb.SingleDeviceMuonWithAuxAdam([dict(params=ours, use_muon=False)])
+            _give_grads(ours, 1)
+            run.step()
+            opt = mb.AdamW(ours)
+            opt.load_state_dict(run.state_dict())
+            assert "use_muon" not in opt.param_groups[0] and [opt.state[p]["step"] for p in ours] == [1, 1]
+            assert [opt.state[p]["moment_bits"] for p in ours] == ([8, 32] if moments == "8bit" else [32, 32])
+            opt.step()
+    finally:
+        mb.set_adam_moments()
+
+
+def test_state_that_means_something_else_is_refused(backend):
+    """Before anything changes."""
+    import muon_b200 as mb
+    theirs, ours = _two_runs(3)
+    opt = mb.AdamW(ours, lr=5e-4)
+    _give_grads(ours, 1)
+    opt.step()
+    for run, match in ((torch.optim.AdamW(theirs, amsgrad=True), "amsgrad"), (torch.optim.AdamW(theirs, maximize=True), "maximize"),
+                       (torch.optim.Adam(theirs, weight_decay=0.1), "decoupled"), (torch.optim.SGD(theirs, momentum=0.9), "betas"),
+                       (torch.optim.Adamax(theirs), "exp_inf"), (mb.SingleDeviceMuon(theirs[:1]), "betas")):
+        _give_grads(theirs, 1)
+        if not isinstance(run, mb.SingleDeviceMuon):
+            run.step()
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(run.state_dict())
+        assert opt.param_groups[0]["lr"] == 5e-4 and [opt.state[p]["step"] for p in ours] == [1, 1]
+    plain = torch.optim.Adam(theirs)  # without decay the two are the same
+    _give_grads(theirs, 1)
+    plain.step()
+    opt.load_state_dict(plain.state_dict())
+    opt.step()
+    assert [opt.state[p]["step"] for p in ours] == [2, 2]
+
+
+def test_torch_state_of_dtensors(backend, tmp_path):
+    """torch keeps DTensors as moments, this class the local parts."""
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Shard
+    import muon_b200 as mb
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/pg", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cpu", (1,))
+        make = lambda: torch.nn.Parameter(DTensor.from_local(torch.ones(8, 4), mesh, [Shard(0)]))  # noqa: E731
+        a, b = make(), make()
+        for p in (a, b):
+            p.grad = DTensor.from_local(torch.arange(32.0).view(8, 4), mesh, [Shard(0)])
+        run, opt = torch.optim.AdamW([a]), mb.AdamW([b])
+        run.step()
+        opt.load_state_dict(run.state_dict())
+        assert type(opt.state[b]["exp_avg"]) is torch.Tensor
+        assert torch.equal(opt.state[b]["exp_avg"], run.state[a]["exp_avg"].to_local())
+        opt.step()
+    finally:
+        dist.destroy_process_group()
