@@ -160,8 +160,8 @@ def _master_of(p: Tensor) -> Tensor:
 
 def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
                  grad_scale: Tensor | None = None, seed: int = 0) -> None:
-    """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out and
-    its step already counted: one call per combination of types and device."""
+    """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out: one call
+    per combination of types and device. A state's step is counted when its call has been made."""
     kinds: "OrderedDict[tuple, list]" = OrderedDict()
     for p, g, state in entries:
         if g.stride() != p.stride():  # a gradient in another order of dimensions than its parameter
@@ -176,7 +176,9 @@ def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, fl
         if bits == 8:
             more["seed"] = seed
         (adamw8_step if bits == 8 else adamw_step)([p for p, _, _ in members], [g for _, g, _ in members], *lists,
-                                                   [state["step"] for state in states], **more)
+                                                   [state["step"] + 1 for state in states], **more)
+        for state in states:
+            state["step"] += 1
 
 
 def convert_moments(states: Sequence[dict], bits: int) -> None:
@@ -366,7 +368,6 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
                 if len(state) == 0:
                     bits = 8 if group["state_bits"] == 8 and local.numel() >= group["min_8bit_numel"] else 32
                     new_moments(state, local, bits, group["master_weights"] and local.dtype != torch.float32)
-                state["step"] += 1
             moments_step(entries, float(group["lr"]), float(group["weight_decay"]), tuple(map(float, group["betas"])),
                          float(group["eps"]), factor, int(group["seed"]))
         return loss

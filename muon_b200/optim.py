@@ -82,7 +82,8 @@ def _adam_update_params(optimizer, group) -> None:
                 state["step"] = 0
             else:
                 new_moments(state, p, 8 if moments == "8bit" and p.numel() >= _MIN_8BIT_NUMEL else 32)
-        state["step"] += 1
+        if "moment_bits" not in state:  # (moments_step counts the others)
+            state["step"] += 1
     own = [p for p in params if "moment_bits" in optimizer.state[p]]  # moments in float32 or 8 bits
     if own:
         moments_step([(p, p.grad, optimizer.state[p]) for p in own], group["lr"], group["weight_decay"],

@@ -375,3 +375,33 @@ def test_torch_state_of_dtensors(backend, tmp_path):
         opt.step()
     finally:
         dist.destroy_process_group()
+
+
+# ------------------------------------------------------------------------------- steps that are refused
+@pytest.mark.parametrize("aux", [False, True])
+def test_a_refused_step_is_not_counted(backend, aux):
+    """The step number counts the steps that were taken: a call that refuses its lists leaves it. What the calls
+    before it in the same step() did stays done, and counted."""
+    import muon_b200 as mb
+    params = _params(5)[:2]
+    _give_grads(params, 1)
+    if aux:
+        mb.set_adam_moments("8bit")
+        opt = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)])
+    else:
+        opt = mb.AdamW(params, state_bits=8)
+
+    def refuse(*args):
+        raise ValueError("refused")
+
+    try:
+        opt.step()
+        kept, backend.adamw_step = backend.adamw_step, refuse
+        with pytest.raises(ValueError, match="refused"):
+            opt.step()
+        assert [opt.state[p]["step"] for p in params] == [2, 1]  # (the 8-bit call comes first)
+        backend.adamw_step = kept
+        opt.step()
+        assert [opt.state[p]["step"] for p in params] == [3, 2]
+    finally:
+        mb.set_adam_moments()
