@@ -158,13 +158,18 @@ def _master_of(p: Tensor) -> Tensor:
     return p.detach().to(torch.float32, copy=True, memory_format=torch.preserve_format)
 
 
+def _same_order(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors of one shape have their elements in the same order (dimensions of size 1 have none)."""
+    return a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
                  grad_scale: Tensor | None = None, seed: int = 0) -> None:
     """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out: one call
     per combination of types and device. A state's step is counted when its call has been made."""
     kinds: "OrderedDict[tuple, list]" = OrderedDict()
     for p, g, state in entries:
-        if g.stride() != p.stride():  # a gradient in another order of dimensions than its parameter
+        if not _same_order(g, p):
             wait_for_mark(g)
             g = torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
         kinds.setdefault((p.dtype, g.dtype, p.device, state["moment_bits"], "master" in state), []).append((p, g, state))
@@ -213,7 +218,7 @@ def restore_moments(p: Tensor, saved: dict) -> dict:
     laid_out = keep["exp_avg_codes" if saved["moment_bits"] == 8 else "exp_avg"]
     if laid_out.shape != p.shape:
         raise ValueError(f"moments of shape {tuple(laid_out.shape)} for a parameter of shape {tuple(p.shape)}")
-    if laid_out.stride() == p.stride():
+    if _same_order(laid_out, p):
         return keep
     state = {"moment_bits": saved["moment_bits"], **keep}
     convert_moments([state], 32)

@@ -34,6 +34,14 @@ const char* type_names(int mask) {
   return mask == kF32 ? "float32" : mask == kU8 ? "uint8" : "float32, bfloat16 or float16";
 }
 
+// Whether two tensors have one shape and their elements in one order (dimensions of size 1 have none).
+bool same_order(const at::Tensor& a, const at::Tensor& b) {
+  if (a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) != 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
 struct Ref {  // owned reference
   PyObject* p;
   explicit Ref(PyObject* o = nullptr) : p(o) {}
@@ -127,7 +135,7 @@ struct Lists {
         }
         dense = t.is_contiguous() && (layout == kScales || ref.is_contiguous());
         if (!dense && layout == kLikeFirst)  // the first list's tensor is dense
-          dense = t.sizes() == ref.sizes() && t.strides() == ref.strides();
+          dense = same_order(t, ref);
       }
       if (!dense && size > 1) {
         PyErr_Format(PyExc_ValueError, "%s: %s tensors must be contiguous, or dense with the strides of the tensor they "

@@ -70,9 +70,6 @@ def _adam_update_params(optimizer, group) -> None:
     for p in params:
         if p.grad is None:
             p.grad = torch.zeros_like(p)
-        elif not p.grad.is_contiguous():
-            wait_for_mark(p.grad)
-            p.grad = p.grad.contiguous()
         state = optimizer.state[p]
         if len(state) == 0:
             moments = get_adam_moments()
@@ -82,7 +79,10 @@ def _adam_update_params(optimizer, group) -> None:
                 state["step"] = 0
             else:
                 new_moments(state, p, 8 if moments == "8bit" and p.numel() >= _MIN_8BIT_NUMEL else 32)
-        if "moment_bits" not in state:  # (moments_step counts the others)
+        if "moment_bits" not in state:  # (moments_step counts the others, and takes gradients in the parameter's order)
+            if not p.grad.is_contiguous():
+                wait_for_mark(p.grad)
+                p.grad = p.grad.contiguous()
             state["step"] += 1
     own = [p for p in params if "moment_bits" in optimizer.state[p]]  # moments in float32 or 8 bits
     if own:

@@ -405,3 +405,72 @@ def test_a_refused_step_is_not_counted(backend, aux):
         assert [opt.state[p]["step"] for p in params] == [3, 2]
     finally:
         mb.set_adam_moments()
+
+
+# ------------------------------------------------------------------------------- order of memory
+def _like(x, order):
+    """A copy of x whose memory has these strides."""
+    out = torch.empty_strided(x.shape, order)
+    return out.copy_(x)
+
+
+# shape, strides of the parameter, strides of the gradient: sizes of 1 have no order
+_SAME_ORDER = [((96, 64, 1, 1), (64, 1, 1, 1), (64, 1, 64, 64)), ((96, 64, 1, 1), (64, 1, 64, 64), (64, 1, 1, 1)),
+               ((1, 80, 64), (5120, 64, 1), (7, 64, 1)), ((64, 24, 3, 1), (72, 1, 24, 24), (72, 1, 24, 72))]
+
+
+@pytest.mark.parametrize("shape,of_p,of_g", _SAME_ORDER)
+@pytest.mark.parametrize("aux", [False, True])
+def test_sizes_of_one_have_no_order(backend, shape, of_p, of_g, aux):
+    """The gradient is handed over as it is, and moments saved for one such parameter are loaded for another code for
+    code."""
+    import muon_b200 as mb
+    gen = torch.Generator().manual_seed(7)
+    seen = []
+
+    def step(ps, gs, mc, msc, vc, vsc, *rest):  # (the stand-in's own takes contiguous codes only)
+        seen.extend(g.data_ptr() for g in gs)
+        for codes in mc + vc:
+            codes.copy_(torch.randint(0, 256, shape, generator=gen))
+
+    backend.adamw8_step = step
+
+    def make(order):
+        p = torch.nn.Parameter(_like(torch.ones(shape), order))
+        if aux:
+            return p, mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=False)])
+        return p, mb.AdamW([p], state_bits=8)
+
+    try:
+        if aux:
+            mb.set_adam_moments("8bit")
+        p, opt = make(of_p)
+        q, again = make(of_g)
+        p.grad = _like(torch.randn(shape, generator=gen), of_g)
+        opt.step()
+        assert seen == [p.grad.data_ptr()]
+        again.load_state_dict(opt.state_dict())
+        for key in ("exp_avg_codes", "exp_avg_sq_codes"):
+            assert torch.equal(again.state[q][key], opt.state[p][key]), key
+    finally:
+        mb.set_adam_moments()
+
+
+def test_channels_last_gradients_of_the_auxiliary_adam_are_not_copied(backend):
+    import muon_b200 as mb
+    p = torch.nn.Parameter(torch.ones(64, 24, 3, 3).to(memory_format=torch.channels_last))
+    seen = []
+    backend.adamw_step = lambda ps, gs, *rest: seen.extend(g.data_ptr() for g in gs)
+    try:
+        mb.set_adam_moments("fp32")
+        opt = mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=False)])
+        p.grad = torch.randn(64, 24, 3, 3).to(memory_format=torch.channels_last)
+        grad = p.grad
+        opt.step()
+        opt.step()
+    finally:
+        mb.set_adam_moments()
+    assert p.grad is grad and seen == [grad.data_ptr()] * 2
+    backend.adam_step = lambda ps, gs, *rest: seen.extend(g.is_contiguous() for g in gs)
+    mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=False)]).step()  # the parameter's type: as before
+    assert seen[-1] is True

@@ -105,3 +105,28 @@ def test_norm_and_step_of_marked_gradients_on_two_streams(mb, clip):
     assert ((M[0].cpu().double() - want).abs() <= 10.5 * 2.0 ** -24 * want.abs() + 1e-44).all()
     from muon_b200 import engine
     assert not engine._grad_ready
+
+
+# ------------------------------------------------------------------------------------ order of memory
+@pytest.mark.parametrize("shape,of_p,of_g", [((96, 64, 1, 1), (64, 1, 1, 1), (64, 1, 64, 64)),
+                                             ((64, 24, 3, 1), (72, 1, 24, 24), (72, 1, 24, 72)),
+                                             ((1, 24, 3, 64), (7, 1, 24, 72), (4608, 1, 24, 72))])
+def test_lists_whose_sizes_of_one_have_other_strides(mb, shape, of_p, of_g):
+    """The elements are in one order, so the call takes them; every other difference of strides is refused."""
+    gen = torch.Generator().manual_seed(32)
+    p, g = torch.randn(shape, generator=gen), torch.randn(shape, generator=gen)
+    place = lambda x, order: torch.empty_strided(shape, order, device="cuda").copy_(x)  # noqa: E731
+    P, G, M, V = place(p, of_p), place(g, of_g), place(p * 0, of_g), place(p * 0, of_p)
+    mb.adamw_step([P], [G], [M], [V], 1, lr=1e-2, weight_decay=0.1)
+    args = (p, g, p * 0, p * 0, 1, 1e-2, (0.9, 0.999), 1e-8, 0.1)
+    tol = orc.adamw_tolerance(*args)
+    for got, want, t in zip((P, M, V), orc.adamw64(*args), tol):
+        assert ((got.cpu().double() - want).abs() <= t).all()
+    codes, scales = mb.quantize_state([M], "exp_avg")
+    out = [place(p, of_g)]
+    mb.dequantize_state(codes, scales, "exp_avg", out=out)
+    want = orc.dequantize(*orc.quantize(torch.as_strided(M, (M.numel(),), (1,)).cpu(), "exp_avg"), "exp_avg")
+    assert torch.equal(torch.as_strided(out[0], (M.numel(),), (1,)).cpu(), want)
+    if not P.is_contiguous():
+        with pytest.raises(ValueError, match="strides"):
+            mb.adamw_step([P], [G.contiguous()], [M], [V], 2)
