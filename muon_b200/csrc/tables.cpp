@@ -45,6 +45,7 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
 struct Ref {  // owned reference
   PyObject* p;
   explicit Ref(PyObject* o = nullptr) : p(o) {}
+  Ref(Ref&& other) noexcept : p(other.release()) {}
   Ref(const Ref&) = delete;
   Ref& operator=(const Ref&) = delete;
   ~Ref() { Py_XDECREF(p); }
@@ -64,7 +65,8 @@ struct Lists {
   std::vector<int64_t> numel;
   std::vector<int> codes;  // element types of the first list
   std::vector<Range> written, read;
-  Ref first;
+  std::vector<at::TensorImpl*> changed;
+  std::vector<Ref> held;  // the lists themselves (one made of an iterator's tensors may be all that holds them)
 
   explicit Lists(const char* w) : what(w) {}
 
@@ -73,7 +75,7 @@ struct Lists {
     Ref fast(PySequence_Fast(tensors, "lists of tensors are lists or tuples"));
     if (!fast.p) return false;
     const Py_ssize_t count = PySequence_Fast_GET_SIZE(fast.p);
-    const bool is_first = first.p == nullptr;
+    const bool is_first = held.empty();
     if (is_first) {
       n = count;
       numel.resize(n);
@@ -86,6 +88,7 @@ struct Lists {
     found = 0;
     std::vector<Range> ranges;
     ranges.reserve(n);
+    if (writes) changed.reserve(changed.size() + n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
       if (!THPVariable_Check(o)) {
@@ -125,7 +128,7 @@ struct Lists {
         codes[i] = type_code(bit);
         dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
       } else {
-        const at::Tensor& ref = THPVariable_Unpack(PySequence_Fast_GET_ITEM(first.p, i));
+        const at::Tensor& ref = THPVariable_Unpack(PySequence_Fast_GET_ITEM(held[0].p, i));
         const int64_t want =
             layout == kLikeFirst ? numel[i] : (numel[i] + MUON_B200_STATE_BLOCK - 1) / MUON_B200_STATE_BLOCK;
         if (size != want) {
@@ -143,12 +146,13 @@ struct Lists {
         return false;
       }
       table[i] = size == 0 ? nullptr : writes ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
+      if (writes && !t.is_inference()) changed.push_back(t.unsafeGetTensorImpl());
       if (size > 0) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(table[i]);
         ranges.emplace_back(at, at + size * t.element_size());
       }
     }
-    if (is_first) first.p = fast.release();
+    held.push_back(std::move(fast));
     if (!writes) {
       read.insert(read.end(), ranges.begin(), ranges.end());
     } else if (!merge(ranges)) {
@@ -170,6 +174,13 @@ struct Lists {
       }
     }
     return true;
+  }
+
+  // After the library's call: autograd learns that the tensors have new values, as it does from torch's functions.
+  int done(int rc) const {
+    if (rc == 0)
+      for (at::TensorImpl* t : changed) t->bump_version();
+    return rc;
   }
 
   // Sorted `more` into the sorted written ranges; false when two overlap. Lists mostly come in ascending
@@ -270,7 +281,7 @@ PyObject* adamw(PyObject*, PyObject* args) {
                                           factor, stream)
                        : muon_b200_adamw(p.data(), wp, g.data(), m[0].data(), m[1].data(), lists.numel.data(),
                                          steps.data(), n, code, grad_code, lr, wd, b1, b2, eps, factor, stream);
-  return PyLong_FromLong(rc);
+  return PyLong_FromLong(lists.done(rc));
   END_HANDLE_TH_ERRORS
 }
 
@@ -294,8 +305,10 @@ PyObject* convert(PyObject*, PyObject* args) {
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   const int n = static_cast<int>(lists.n);
-  return PyLong_FromLong(to_codes ? muon_b200_quantize_state(x.data(), c.data(), s.data(), lists.numel.data(), n, code, kind, stream)
-                                  : muon_b200_dequantize_state(c.data(), s.data(), x.data(), lists.numel.data(), n, code, kind, stream));
+  const int rc = to_codes
+      ? muon_b200_quantize_state(x.data(), c.data(), s.data(), lists.numel.data(), n, code, kind, stream)
+      : muon_b200_dequantize_state(c.data(), s.data(), x.data(), lists.numel.data(), n, code, kind, stream);
+  return PyLong_FromLong(lists.done(rc));
   END_HANDLE_TH_ERRORS
 }
 
@@ -327,7 +340,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
                                              reinterpret_cast<void*>(at), bytes, stream)
                       : muon_b200_grad_norm(x.data(), lists.numel.data(), lists.codes.data(), n, max_norm, result,
                                             reinterpret_cast<void*>(at), bytes, stream);
-  return Py_BuildValue("iNN", rc, THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.select(0, 1)));
+  return Py_BuildValue("iNN", lists.done(rc), THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.select(0, 1)));
   END_HANDLE_TH_ERRORS
 }
 
