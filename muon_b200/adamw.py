@@ -163,15 +163,21 @@ def _same_order(a: Tensor, b: Tensor) -> bool:
     return a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
 
 
+def _in_order_of(g: Tensor, p: Tensor) -> Tensor:
+    """The gradient, or a copy of it with its elements in the order of its parameter's."""
+    if _same_order(g, p):
+        return g
+    wait_for_mark(g)
+    return torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
+
+
 def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
                  grad_scale: Tensor | None = None, seed: int = 0) -> None:
     """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out: one call
     per combination of types and device. A state's step is counted when its call has been made."""
     kinds: "OrderedDict[tuple, list]" = OrderedDict()
     for p, g, state in entries:
-        if not _same_order(g, p):
-            wait_for_mark(g)
-            g = torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
+        g = _in_order_of(g, p)
         kinds.setdefault((p.dtype, g.dtype, p.device, state["moment_bits"], "master" in state), []).append((p, g, state))
     for (_, _, _, bits, master), members in kinds.items():
         states = [state for _, _, state in members]
@@ -357,6 +363,8 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
                         wait_for_mark(g)
                         g = g.redistribute(placements=p.placements)
                     g = g.to_local()
+                if self.max_grad_norm is not None:  # the norm takes dense gradients
+                    g = _in_order_of(g, local)
                 entries.append((local, g, self.state[p]))
             if entries:
                 work.append((group, entries))

@@ -474,3 +474,25 @@ def test_channels_last_gradients_of_the_auxiliary_adam_are_not_copied(backend):
     backend.adam_step = lambda ps, gs, *rest: seen.extend(g.is_contiguous() for g in gs)
     mb.SingleDeviceMuonWithAuxAdam([dict(params=[p], use_muon=False)]).step()  # the parameter's type: as before
     assert seen[-1] is True
+
+
+def test_clipping_takes_the_gradients_that_a_step_takes(backend):
+    """A gradient that is a slice of a larger buffer, or one value for all elements, is copied into its
+    parameter's order: with clipping before the norm, which needs dense memory."""
+    import muon_b200 as mb
+    gen = torch.Generator().manual_seed(8)
+    plain = backend.grad_norm
+
+    def norm(tensors, max_norm, clip):
+        assert all(t.is_contiguous() for t in tensors)
+        return plain(tensors, max_norm, clip)
+
+    backend.grad_norm = norm
+    results = []
+    for max_norm in (None, 1e9):
+        params = [torch.nn.Parameter(torch.ones(6, 10)), torch.nn.Parameter(torch.ones(7))]
+        params[0].grad = torch.arange(120.0).view(6, 20)[:, ::2]
+        params[1].grad = torch.full((1,), 0.5).expand(7)
+        mb.AdamW(params, max_grad_norm=max_norm).step()
+        results.append(params)
+    assert all(torch.equal(p, q) for p, q in zip(*results))
