@@ -59,7 +59,8 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg_codes
 
 
 def _gradients(tensors) -> list[Tensor]:
-    """The gradients of parameters (those that have one), or the tensors themselves."""
+    """The gradients of parameters (those that have one; a plain leaf that requires gradients is a parameter too),
+    or the tensors themselves."""
     return gradients([tensors] if isinstance(tensors, Tensor) else tensors)
 
 

@@ -352,10 +352,14 @@ PyObject* gradients(PyObject*, PyObject* tensors) {
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast.p);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
-    int parameter = 0;  // (a plain torch.Tensor is none; a subclass may be one without being its subtype)
+    int parameter = 0;  // (a subclass of torch.Tensor may be one without being its subtype)
     if (Py_TYPE(o) == reinterpret_cast<PyTypeObject*>(ParameterClass)) parameter = 1;
     else if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass)) parameter = PyObject_IsInstance(o, ParameterClass);
     if (parameter < 0) return nullptr;
+    if (!parameter && THPVariable_Check(o)) {  // or a plain leaf: an optimizer takes those too
+      const at::Tensor& t = THPVariable_Unpack(o);
+      parameter = t.requires_grad() && t.is_leaf();
+    }
     Ref g(parameter ? PyObject_GetAttrString(o, "grad") : Py_NewRef(o));
     if (!g.p || (g.p != Py_None && PyList_Append(out.p, g.p) < 0)) return nullptr;
   }

@@ -81,7 +81,7 @@ def mark_grad_ready(tensor: Tensor, event: "torch.cuda.Event | None" = None) -> 
     in flight. Gradients without a mark are assumed ready in the order of step()'s own stream,
     which is the reference's behaviour. A mark is consumed by the step that uses it; a norm taken before waits
     for it and leaves it, and clipping moves it behind the scaled values."""
-    if isinstance(tensor, torch.nn.Parameter):
+    if isinstance(tensor, torch.nn.Parameter) or (tensor.requires_grad and tensor.is_leaf):
         if tensor.grad is None:
             raise ValueError("mark_grad_ready: the parameter has no gradient yet; allocate p.grad (or pass "
                              "the gradient tensor itself) before marking it")

@@ -496,3 +496,25 @@ def test_clipping_takes_the_gradients_that_a_step_takes(backend):
         mb.AdamW(params, max_grad_norm=max_norm).step()
         results.append(params)
     assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+def test_a_parameter_may_be_a_plain_leaf(streams, monkeypatch):
+    """As for torch.optim and torch.nn.utils: a tensor that requires gradients of its own is a parameter, and its
+    .grad is meant (clip_grad_norm_ must not scale the weights). A gradient that has a graph behind it is none."""
+    from muon_b200 import engine
+    from muon_b200._tables import gradients
+    import muon_b200 as mb
+    leaf = torch.ones(3, requires_grad=True)
+    parameter, plain = torch.nn.Parameter(torch.ones(3)), torch.ones(3)
+    frozen = torch.nn.Parameter(torch.ones(3), requires_grad=False)
+    assert gradients([leaf, parameter, frozen]) == []
+    leaf.grad, parameter.grad = torch.full((3,), 2.0), torch.full((3,), 3.0)
+    with_graph = leaf * 2
+    got = gradients([leaf, plain, with_graph, parameter, frozen])
+    assert len(got) == 4 and all(a is b for a, b in zip(got, (leaf.grad, plain, with_graph, parameter.grad)))
+    monkeypatch.setattr(engine, "_require_cuda", lambda *args: None)
+    mb.mark_grad_ready(leaf)
+    assert list(engine._grad_ready) == [leaf.grad.data_ptr()]
+    leaf.grad = None
+    with pytest.raises(ValueError, match="no gradient"):
+        mb.mark_grad_ready(leaf)
