@@ -132,6 +132,15 @@ def _load() -> ctypes.CDLL:
 
 lib = _load()
 
+try:  # (its libraries are torch's, loaded with torch)
+    import torch  # noqa: F401
+
+    from . import _tables  # noqa: F401
+except ImportError as error:
+    raise ImportError(
+        f"{os.path.join(_PKG_DIR, '_tables.so')} is missing or does not load with this torch and Python ({error}). "
+        "Build it with `python muon_b200/build.py` (needs nvcc and a C++ compiler).") from error
+
 
 def check(rc: int) -> None:
     if rc != 0:

@@ -6,6 +6,7 @@ package needs the library to exist already. nvcc cross-compiles, so no GPU is ne
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -19,6 +20,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libmuon_b200.so")
 TABLES_PATH = os.path.join(PKG_DIR, "_tables.so")
+TABLES_STAMP = TABLES_PATH + ".built"  # what it was built for
 SOURCES = ("api.cu", "ns_driver.cu", "ns_gemm.cu", "elementwise.cu", "adamw.cu", "profiling.cu", "peer.cu", "no_alloc.cu")
 HEADERS = ("common.cuh", "ns_driver.h", "ns_gemm.h", "elementwise.h", "adamw.h", "profiling.h", os.path.join("..", "..", "include", "muon_b200.h"))
 TABLES_SOURCES = ("tables.cpp", os.path.join("..", "..", "include", "muon_b200.h"))
@@ -44,8 +46,27 @@ def _older(target: str, names) -> bool:
     return any(os.path.getmtime(d) > built for d in deps if os.path.exists(d))
 
 
+def _torch_dir() -> str:
+    spec = importlib.util.find_spec("torch")  # the path alone: torch need not be imported to build
+    if spec is None or not spec.submodule_search_locations:
+        raise RuntimeError("PyTorch not found: cannot build _tables.so")
+    return list(spec.submodule_search_locations)[0]
+
+
+def _tables_target() -> str:
+    """The torch and the Python that _tables.so is bound to."""
+    return f"torch {importlib.metadata.version('torch')} in {_torch_dir()}, {sys.implementation.cache_tag}\n"
+
+
+def _tables_stale() -> bool:
+    if _older(TABLES_PATH, TABLES_SOURCES) or not os.path.exists(TABLES_STAMP):
+        return True
+    with open(TABLES_STAMP) as f:
+        return f.read() != _tables_target()
+
+
 def is_stale() -> bool:
-    return _older(LIB_PATH, SOURCES + HEADERS) or _older(TABLES_PATH, TABLES_SOURCES)
+    return _older(LIB_PATH, SOURCES + HEADERS) or _tables_stale()
 
 
 def _run(cmd, verbose: bool = False) -> None:
@@ -59,10 +80,7 @@ def _run(cmd, verbose: bool = False) -> None:
 
 
 def _build_tables(verbose: bool) -> None:
-    spec = importlib.util.find_spec("torch")  # the path alone: torch need not be imported to build
-    if spec is None or not spec.submodule_search_locations:
-        raise RuntimeError("PyTorch not found: cannot build _tables.so")
-    torch_dir = list(spec.submodule_search_locations)[0]
+    torch_dir = _torch_dir()
     include = os.path.join(torch_dir, "include")
     compiler = shutil.which("g++") or shutil.which("c++")
     if compiler is None:
@@ -75,10 +93,13 @@ def _build_tables(verbose: bool) -> None:
           "-o", TABLES_PATH, os.path.join(CSRC, TABLES_SOURCES[0]),
           "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
           "-L" + PKG_DIR, "-lmuon_b200", "-Wl,-rpath,$ORIGIN"], verbose)
+    with open(TABLES_STAMP, "w") as f:
+        f.write(_tables_target())
 
 
 def build_library(force: bool = False, verbose: bool = False) -> str:
-    """Compile what is missing or older than its sources, files side by side. Returns the library's path."""
+    """Compile what is missing, older than its sources or made for another torch, files side by side. Returns the
+    library's path."""
     jobs = []
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor() as pool:
         objects = []
@@ -92,7 +113,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             job.result()
         if objects:
             _run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects], verbose)
-    if force or _older(TABLES_PATH, TABLES_SOURCES):
+    if force or _tables_stale():
         _build_tables(verbose)
     return LIB_PATH
 

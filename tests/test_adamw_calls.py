@@ -518,3 +518,59 @@ def test_a_parameter_may_be_a_plain_leaf(streams, monkeypatch):
     leaf.grad = None
     with pytest.raises(ValueError, match="no gradient"):
         mb.mark_grad_ready(leaf)
+
+
+# ------------------------------------------------------------------------------- the build
+def _build_module():
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("_build", os.path.join(_package(), "build.py"))
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
+def _package():
+    import os
+    import muon_b200
+    return os.path.dirname(muon_b200.__file__)
+
+
+def test_the_extension_is_built_again_for_another_torch(tmp_path):
+    """_tables.so is bound to the torch and the Python it was built for, whose files are newer or older than it."""
+    build = _build_module()
+    built = []
+    build._run = lambda cmd, verbose=False: built.append(cmd)
+    build._older = lambda target, names: False
+    stamp = build.TABLES_STAMP = str(tmp_path / "stamp")
+    assert build.is_stale()  # nothing says what it was built for
+    build.build_library()
+    assert len(built) == 1 and any("tables.cpp" in x for x in built[0])
+    assert not build.is_stale()
+    build.build_library()
+    assert len(built) == 1
+    with open(stamp) as f:
+        text = f.read()
+    assert torch.__version__ in text
+    with open(stamp, "w") as f:
+        f.write(text.replace(torch.__version__, "1.0"))
+    assert build.is_stale()
+    build.build_library()
+    assert len(built) == 2 and not build.is_stale()
+
+
+def test_an_extension_that_does_not_load_says_what_to_do(tmp_path):
+    import os
+    import subprocess
+    import sys
+    package = tmp_path / "muon_b200"
+    package.mkdir()
+    for name in os.listdir(_package()):
+        if name.endswith(".py") or name == "libmuon_b200.so":
+            os.symlink(os.path.join(_package(), name), package / name)
+    for content in (None, b"no library"):
+        if content is not None:
+            (package / "_tables.so").write_bytes(content)
+        out = subprocess.run([sys.executable, "-c", "import muon_b200"], cwd=tmp_path, capture_output=True, text=True,
+                             env={**os.environ, "PYTHONPATH": str(tmp_path)})
+        assert out.returncode != 0 and "python muon_b200/build.py" in out.stderr and "_tables.so" in out.stderr
