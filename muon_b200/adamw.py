@@ -161,12 +161,12 @@ def _master_of(p: Tensor) -> Tensor:
 
 def _same_order(a: Tensor, b: Tensor) -> bool:
     """Whether two tensors of one shape have their elements in the same order (dimensions of size 1 have none)."""
-    return a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
 
 
-def _in_order_of(g: Tensor, p: Tensor) -> Tensor:
+def in_order_of(g: Tensor, p: Tensor) -> Tensor:
     """The gradient, or a copy of it with its elements in the order of its parameter's."""
-    if _same_order(g, p):
+    if g.stride() == p.stride() or _same_order(g, p):
         return g
     wait_for_mark(g)
     return torch.empty_like(p, dtype=g.dtype, memory_format=torch.preserve_format).copy_(g)
@@ -174,23 +174,23 @@ def _in_order_of(g: Tensor, p: Tensor) -> Tensor:
 
 def moments_step(entries, lr: float, weight_decay: float, betas: tuple[float, float], eps: float,
                  grad_scale: Tensor | None = None, seed: int = 0) -> None:
-    """One step for a list of (parameter, gradient, state), state as ``new_moments`` lays it out: one call
-    per combination of types and device. A state's step is counted when its call has been made."""
+    """One step for a list of (parameter, gradient in its order, state), state as ``new_moments`` lays it out: one
+    call per combination of types and device. A state's step is counted when its call has been made."""
     kinds: "OrderedDict[tuple, list]" = OrderedDict()
     for p, g, state in entries:
-        g = _in_order_of(g, p)
         kinds.setdefault((p.dtype, g.dtype, p.device, state["moment_bits"], "master" in state), []).append((p, g, state))
     for (_, _, _, bits, master), members in kinds.items():
         states = [state for _, _, state in members]
+        steps = [state["step"] + 1 for state in states]
         lists = [[state[key] for state in states] for key in _MOMENT_KEYS[bits]]
         more = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, grad_scale=grad_scale,
                     masters=[state["master"] for state in states] if master else None)
         if bits == 8:
             more["seed"] = seed
         (adamw8_step if bits == 8 else adamw_step)([p for p, _, _ in members], [g for _, g, _ in members], *lists,
-                                                   [state["step"] + 1 for state in states], **more)
-        for state in states:
-            state["step"] += 1
+                                                   steps, **more)
+        for state, now in zip(states, steps):
+            state["step"] = now
 
 
 def convert_moments(states: Sequence[dict], bits: int) -> None:
@@ -364,9 +364,7 @@ class AdamW(KeepsMomentTypes, torch.optim.Optimizer):
                         wait_for_mark(g)
                         g = g.redistribute(placements=p.placements)
                     g = g.to_local()
-                if self.max_grad_norm is not None:  # the norm takes dense gradients
-                    g = _in_order_of(g, local)
-                entries.append((local, g, self.state[p]))
+                entries.append((local, in_order_of(g, local), self.state[p]))
             if entries:
                 work.append((group, entries))
         if not work:

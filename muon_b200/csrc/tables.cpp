@@ -55,23 +55,42 @@ struct Ref {  // owned reference
 using Range = std::pair<uintptr_t, uintptr_t>;
 using Table = std::vector<void*>;
 enum Layout { kLikeFirst, kScales };  // sizes of a list: those of the first list, or one per block of its elements
+// What a call does with a list. kUpdates: writes tensors that a backward pass may have saved, and counts a version of
+// them as torch's in-place functions do. Moments, masters, codes and scales are state that nothing but a step reads: kWrites
+// (counting a version takes 13 ns a tensor, a third of what the tensor takes in all).
+enum Use { kReads, kWrites, kUpdates };
 
 // The lists of one call. All tensors are on one device; what is written overlaps nothing else of the call (tensors
 // that are only read may share memory).
 struct Lists {
+  // Part of the memory of a list: ranges[first .. last), all of it in [low, high). Lists mostly come in a few runs
+  // that ascend, from as many segments of the allocator.
+  struct Run {
+    size_t first, last;
+    uintptr_t low, high;
+    bool written;
+    bool ordered;  // ascending or descending, and apart from one another
+  };
+  static constexpr size_t kMostRuns = 24;
   const char* what;
   Py_ssize_t n = 0;
   int64_t device = -1;
   std::vector<int64_t> numel;
   std::vector<int> codes;  // element types of the first list
-  std::vector<Range> written, read;
+  std::vector<Range> ranges;
+  std::vector<Run> runs;
   std::vector<at::TensorImpl*> changed;
   std::vector<Ref> held;  // the lists themselves (one made of an iterator's tensors may be all that holds them)
 
-  explicit Lists(const char* w) : what(w) {}
+  const int most;  // lists, at most; 0: one, and nothing is written
+
+  Lists(const char* w, int most_lists) : what(w), most(most_lists) {
+    held.reserve(7);
+    if (most > 0) runs.reserve(kMostRuns + most + 1);
+  }
 
   // Adds a list; false with a Python error set. `found`: mask of the types in it.
-  bool add(const char* name, PyObject* tensors, int types, Layout layout, bool writes, Table& table, int& found) {
+  bool add(const char* name, PyObject* tensors, int types, Layout layout, Use use, Table& table, int& found) {
     Ref fast(PySequence_Fast(tensors, "lists of tensors are lists or tuples"));
     if (!fast.p) return false;
     const Py_ssize_t count = PySequence_Fast_GET_SIZE(fast.p);
@@ -80,15 +99,16 @@ struct Lists {
       n = count;
       numel.resize(n);
       codes.resize(n);
+      if (most > 0) ranges.reserve(most * n + 1);
     } else if (count != n) {
       PyErr_Format(PyExc_ValueError, "%s: %zd %s tensors for %zd tensors", what, count, name, n);
       return false;
     }
     table.resize(n);
     found = 0;
-    std::vector<Range> ranges;
-    ranges.reserve(n);
-    if (writes) changed.reserve(changed.size() + n);
+    const bool writes = use != kReads;
+    const size_t begin = ranges.size();
+    if (use == kUpdates) changed.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PySequence_Fast_GET_ITEM(fast.p, i);
       if (!THPVariable_Check(o)) {
@@ -146,25 +166,57 @@ struct Lists {
         return false;
       }
       table[i] = size == 0 ? nullptr : writes ? t.mutable_data_ptr() : const_cast<void*>(t.const_data_ptr());
-      if (writes && !t.is_inference()) changed.push_back(t.unsafeGetTensorImpl());
-      if (size > 0) {
+      if (use == kUpdates && !t.is_inference()) changed.push_back(t.unsafeGetTensorImpl());
+      if (size > 0 && most > 0) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(table[i]);
         ranges.emplace_back(at, at + size * t.element_size());
       }
     }
     held.push_back(std::move(fast));
-    if (!writes) {
-      read.insert(read.end(), ranges.begin(), ranges.end());
-    } else if (!merge(ranges)) {
-      PyErr_Format(PyExc_ValueError, "%s: memory that is written (%s) appears twice in the call", what, name);
-      return false;
-    }
+    add_runs(begin, writes);
     return true;
   }
 
-  // After the last list: false with a Python error set when something that is read lies in what is written.
-  bool reads_are_apart() {
-    if (!std::is_sorted(read.begin(), read.end())) std::sort(read.begin(), read.end());
+  // The ranges from `begin` on: the memory of one list, as runs that ascend or descend.
+  void add_runs(size_t begin, bool written) {
+    for (size_t i = begin; i < ranges.size();) {
+      Run r = {i, i + 1, ranges[i].first, ranges[i].second, written, true};
+      const bool rest = runs.size() + 1 >= kMostRuns;  // too many to compare with one another
+      bool up = true, down = true;
+      for (; r.last < ranges.size(); ++r.last) {
+        const Range &before = ranges[r.last - 1], &now = ranges[r.last];
+        up = up && now.first >= before.second;
+        down = down && now.second <= before.first;
+        if (!up && !down && !rest) break;
+        r.low = std::min(r.low, now.first);
+        r.high = std::max(r.high, now.second);
+      }
+      r.ordered = up || down || !rest;
+      runs.push_back(r);
+      i = r.last;
+    }
+  }
+
+  // After the last list: false with a Python error set when memory that is written appears twice in the call. Runs
+  // that share no span of addresses with another one are apart already; the others are sorted and compared.
+  bool apart() const {
+    std::vector<Range> written, read;
+    for (const Run& r : runs) {
+      bool compare = r.written && !r.ordered;
+      for (const Run& o : runs)
+        compare = compare || (&o != &r && (o.written || r.written) && o.low < r.high && r.low < o.high);
+      if (!compare) continue;
+      std::vector<Range>& to = r.written ? written : read;
+      const size_t middle = to.size();
+      to.insert(to.end(), ranges.begin() + r.first, ranges.begin() + r.last);
+      if (!std::is_sorted(to.begin() + middle, to.end())) std::sort(to.begin() + middle, to.end());
+      std::inplace_merge(to.begin(), to.begin() + middle, to.end());
+    }
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i - 1].second > written[i].first) {
+        PyErr_Format(PyExc_ValueError, "%s: memory that is written appears twice in the call", what);
+        return false;
+      }
     size_t w = 0;  // first written range that ends behind the start of this read one
     for (const Range& r : read) {
       while (w < written.size() && written[w].second <= r.first) ++w;
@@ -181,18 +233,6 @@ struct Lists {
     if (rc == 0)
       for (at::TensorImpl* t : changed) t->bump_version();
     return rc;
-  }
-
-  // Sorted `more` into the sorted written ranges; false when two overlap. Lists mostly come in ascending
-  // order of address, so this is linear.
-  bool merge(std::vector<Range>& more) {
-    if (!std::is_sorted(more.begin(), more.end())) std::sort(more.begin(), more.end());
-    const size_t middle = written.size();
-    written.insert(written.end(), more.begin(), more.end());
-    std::inplace_merge(written.begin(), written.begin() + middle, written.end());
-    for (size_t i = 1; i < written.size(); ++i)
-      if (written[i - 1].second > written[i].first) return false;
-    return true;
   }
 
   // The code of a list that must have one type; -1 with a Python error set.
@@ -237,20 +277,20 @@ PyObject* adamw(PyObject*, PyObject* args) {
     return nullptr;
   const bool eight = PyTuple_GET_SIZE(moments) == 4;
   if (!eight && PyTuple_GET_SIZE(moments) != 2) return PyErr_Format(PyExc_ValueError, "two or four lists of moments");
-  Lists lists(eight ? "adamw8_step" : "adamw_step");
+  Lists lists(eight ? "adamw8_step" : "adamw_step", eight ? 7 : 5);
   Table p, g, w, m[4];
   int p_types = 0, g_types = 0, found = 0;
   const bool has_masters = masters != Py_None;
-  if (!lists.add("parameter", params, kFloats, kLikeFirst, true, p, p_types) ||
-      !lists.add("gradient", grads, kFloats, kLikeFirst, false, g, g_types) ||
-      (has_masters && !lists.add("master", masters, kF32, kLikeFirst, true, w, found)))
+  if (!lists.add("parameter", params, kFloats, kLikeFirst, kUpdates, p, p_types) ||
+      !lists.add("gradient", grads, kFloats, kLikeFirst, kReads, g, g_types) ||
+      (has_masters && !lists.add("master", masters, kF32, kLikeFirst, kWrites, w, found)))
     return nullptr;
   static const char* const names32[] = {"exp_avg", "exp_avg_sq"};
   static const char* const names8[] = {"exp_avg code", "exp_avg scale", "exp_avg_sq code", "exp_avg_sq scale"};
   for (int k = 0; k < (eight ? 4 : 2); ++k) {
     const bool scales = eight && k % 2 == 1;
     if (!lists.add(eight ? names8[k] : names32[k], PyTuple_GET_ITEM(moments, k), eight && !scales ? kU8 : kF32,
-                   scales ? kScales : kLikeFirst, true, m[k], found))
+                   scales ? kScales : kLikeFirst, kWrites, m[k], found))
       return nullptr;
   }
   if (lists.n == 0) return PyLong_FromLong(0);
@@ -269,9 +309,10 @@ PyObject* adamw(PyObject*, PyObject* args) {
       return PyErr_Format(PyExc_ValueError, "%s: grad_scale must be one float32 value on cuda:%lld", lists.what,
                           (long long)lists.device);
     factor = static_cast<const float*>(t->const_data_ptr());
-    lists.read.emplace_back(reinterpret_cast<uintptr_t>(factor), reinterpret_cast<uintptr_t>(factor + 1));
+    lists.ranges.emplace_back(reinterpret_cast<uintptr_t>(factor), reinterpret_cast<uintptr_t>(factor + 1));
+    lists.add_runs(lists.ranges.size() - 1, false);
   }
-  if (!lists.reads_are_apart()) return nullptr;
+  if (!lists.apart()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   void* const* wp = has_masters ? w.data() : nullptr;
@@ -292,16 +333,16 @@ PyObject* convert(PyObject*, PyObject* args) {
   PyObject *values, *codes, *scales;
   int kind, to_codes;
   if (!PyArg_ParseTuple(args, "sOOOip", &what, &values, &codes, &scales, &kind, &to_codes)) return nullptr;
-  Lists lists(what);
+  Lists lists(what, 3);
   Table x, c, s;
   int found = 0, types = 0;
-  if (!lists.add("code", codes, kU8, kLikeFirst, to_codes, c, found) ||
-      !lists.add("scale", scales, kF32, kScales, to_codes, s, found) ||
-      !lists.add("value", values, kFloats, kLikeFirst, !to_codes, x, types))
+  if (!lists.add("code", codes, kU8, kLikeFirst, to_codes ? kWrites : kReads, c, found) ||
+      !lists.add("scale", scales, kF32, kScales, to_codes ? kWrites : kReads, s, found) ||
+      !lists.add("value", values, kFloats, kLikeFirst, to_codes ? kReads : kUpdates, x, types))
     return nullptr;
   if (lists.n == 0) return PyLong_FromLong(0);
   const int code = lists.one_type(types, "value");
-  if (code < 0 || !lists.reads_are_apart()) return nullptr;
+  if (code < 0 || !lists.apart()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   const int n = static_cast<int>(lists.n);
@@ -320,11 +361,12 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   double max_norm;
   int clip;
   if (!PyArg_ParseTuple(args, "OdpO", &tensors, &max_norm, &clip, &scratch)) return nullptr;
-  Lists lists(clip ? "clip_grad_norm_" : "grad_norm");
+  Lists lists(clip ? "clip_grad_norm_" : "grad_norm", clip ? 1 : 0);
   Table x;
   int found = 0;
-  if (!lists.add("gradient", tensors, kFloats, kLikeFirst, clip, x, found)) return nullptr;
+  if (!lists.add("gradient", tensors, kFloats, kLikeFirst, clip ? kUpdates : kReads, x, found)) return nullptr;
   if (lists.n == 0) return PyErr_Format(PyExc_ValueError, "%s: no tensors", lists.what);
+  if (!lists.apart()) return nullptr;
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(lists.device));
   void* stream = c10::cuda::getCurrentCUDAStream().stream();
   Ref held(PyObject_CallFunction(scratch, "LN", (long long)lists.device, PyLong_FromVoidPtr(stream)));

@@ -18,7 +18,7 @@ from collections import OrderedDict
 import torch
 import torch.distributed as dist
 
-from .adamw import _MIN_8BIT_NUMEL, KeepsMomentTypes, get_adam_moments, moments_step, new_moments
+from .adamw import _MIN_8BIT_NUMEL, KeepsMomentTypes, get_adam_moments, in_order_of, moments_step, new_moments
 from .engine import get_backend, plan_launches, view_2d, wait_for_mark
 from .exchange import get_peer_push
 from .ownership import get_ownership, owners
@@ -79,14 +79,14 @@ def _adam_update_params(optimizer, group) -> None:
                 state["step"] = 0
             else:
                 new_moments(state, p, 8 if moments == "8bit" and p.numel() >= _MIN_8BIT_NUMEL else 32)
-        if "moment_bits" not in state:  # (moments_step counts the others, and takes gradients in the parameter's order)
+        if "moment_bits" not in state:  # (moments_step counts the others)
             if not p.grad.is_contiguous():
                 wait_for_mark(p.grad)
                 p.grad = p.grad.contiguous()
             state["step"] += 1
     own = [p for p in params if "moment_bits" in optimizer.state[p]]  # moments in float32 or 8 bits
     if own:
-        moments_step([(p, p.grad, optimizer.state[p]) for p in own], group["lr"], group["weight_decay"],
+        moments_step([(p, in_order_of(p.grad, p), optimizer.state[p]) for p in own], group["lr"], group["weight_decay"],
                      group["betas"], group["eps"])
     by_kind: "OrderedDict[tuple, list]" = OrderedDict()
     for p in params:
