@@ -12,6 +12,7 @@
 #include "../../include/muon_b200.h"
 
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <utility>
 #include <vector>
@@ -45,7 +46,6 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
 struct Ref {  // owned reference
   PyObject* p;
   explicit Ref(PyObject* o = nullptr) : p(o) {}
-  Ref(Ref&& other) noexcept : p(other.release()) {}
   Ref(const Ref&) = delete;
   Ref& operator=(const Ref&) = delete;
   ~Ref() { Py_XDECREF(p); }
@@ -71,30 +71,28 @@ struct Lists {
     bool written;
     bool ordered;  // ascending or descending, and apart from one another
   };
-  static constexpr size_t kMostRuns = 24;
+  static constexpr size_t kMostRuns = 24, kMostLists = 8;  // (seven, and the factor)
   const char* what;
   Py_ssize_t n = 0;
   int64_t device = -1;
   std::vector<int64_t> numel;
   std::vector<int> codes;  // element types of the first list
   std::vector<Range> ranges;
-  std::vector<Run> runs;
+  std::array<Run, kMostRuns + kMostLists> runs;
+  size_t n_runs = 0;
   std::vector<at::TensorImpl*> changed;
-  std::vector<Ref> held;  // the lists themselves (one made of an iterator's tensors may be all that holds them)
-
+  std::array<Ref, kMostLists> held;  // the lists themselves (one made of an iterator's tensors may be all that holds them)
+  int n_held = 0;
   const int most;  // lists, at most; 0: one, and nothing is written
 
-  Lists(const char* w, int most_lists) : what(w), most(most_lists) {
-    held.reserve(7);
-    if (most > 0) runs.reserve(kMostRuns + most + 1);
-  }
+  Lists(const char* w, int most_lists) : what(w), most(most_lists) {}
 
   // Adds a list; false with a Python error set. `found`: mask of the types in it.
   bool add(const char* name, PyObject* tensors, int types, Layout layout, Use use, Table& table, int& found) {
     Ref fast(PySequence_Fast(tensors, "lists of tensors are lists or tuples"));
     if (!fast.p) return false;
     const Py_ssize_t count = PySequence_Fast_GET_SIZE(fast.p);
-    const bool is_first = held.empty();
+    const bool is_first = n_held == 0;
     if (is_first) {
       n = count;
       numel.resize(n);
@@ -172,7 +170,7 @@ struct Lists {
         ranges.emplace_back(at, at + size * t.element_size());
       }
     }
-    held.push_back(std::move(fast));
+    held[n_held++].p = fast.release();
     add_runs(begin, writes);
     return true;
   }
@@ -181,7 +179,7 @@ struct Lists {
   void add_runs(size_t begin, bool written) {
     for (size_t i = begin; i < ranges.size();) {
       Run r = {i, i + 1, ranges[i].first, ranges[i].second, written, true};
-      const bool rest = runs.size() + 1 >= kMostRuns;  // too many to compare with one another
+      const bool rest = n_runs + 1 >= kMostRuns;  // too many to compare with one another
       bool up = true, down = true;
       for (; r.last < ranges.size(); ++r.last) {
         const Range &before = ranges[r.last - 1], &now = ranges[r.last];
@@ -192,7 +190,7 @@ struct Lists {
         r.high = std::max(r.high, now.second);
       }
       r.ordered = up || down || !rest;
-      runs.push_back(r);
+      runs[n_runs++] = r;
       i = r.last;
     }
   }
@@ -201,10 +199,13 @@ struct Lists {
   // that share no span of addresses with another one are apart already; the others are sorted and compared.
   bool apart() const {
     std::vector<Range> written, read;
-    for (const Run& r : runs) {
+    for (size_t k = 0; k < n_runs; ++k) {
+      const Run& r = runs[k];
       bool compare = r.written && !r.ordered;
-      for (const Run& o : runs)
-        compare = compare || (&o != &r && (o.written || r.written) && o.low < r.high && r.low < o.high);
+      for (size_t j = 0; j < n_runs; ++j) {
+        const Run& o = runs[j];
+        compare = compare || (j != k && (o.written || r.written) && o.low < r.high && r.low < o.high);
+      }
       if (!compare) continue;
       std::vector<Range>& to = r.written ? written : read;
       const size_t middle = to.size();
@@ -353,7 +354,7 @@ PyObject* convert(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// grad_norm(tensors, max_norm, clip, scratch) -> (status, norm, factor). scratch(device) returns the address of
+// grad_norm(tensors, max_norm, clip, scratch) -> (status, norm, factor; None with clip). scratch(device) returns the address of
 // muon_b200_grad_norm_scratch_bytes() bytes that this call may use, as an integer.
 PyObject* grad_norm(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -382,7 +383,8 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
                                              reinterpret_cast<void*>(at), bytes, stream)
                       : muon_b200_grad_norm(x.data(), lists.numel.data(), lists.codes.data(), n, max_norm, result,
                                             reinterpret_cast<void*>(at), bytes, stream);
-  return Py_BuildValue("iNN", lists.done(rc), THPVariable_Wrap(out.select(0, 0)), THPVariable_Wrap(out.select(0, 1)));
+  return Py_BuildValue("iNN", lists.done(rc), THPVariable_Wrap(out.select(0, 0)),
+                       clip ? Py_NewRef(Py_None) : THPVariable_Wrap(out.select(0, 1)));
   END_HANDLE_TH_ERRORS
 }
 

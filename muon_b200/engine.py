@@ -559,8 +559,8 @@ class CudaBackend:
             self.launch_groups += 1
 
     # -- AdamW, moments in 32 or 8 bits; gradient norm (adamw.py) --------------------------
-    # _tables checks the lists (one device, element types, sizes, memory order, nothing written twice) and
-    # makes the library call on the current stream of their device.
+    # _tables checks the lists (one device, element types, sizes, memory order, nothing that is written elsewhere in
+    # the call) and makes the library call on the current stream of their device.
     def adamw_step(self, params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor],
                    exp_avg_sqs: Sequence[Tensor], steps, lr: float, weight_decay: float, betas: tuple[float, float],
                    eps: float, masters=None, grad_scale: Tensor | None = None) -> None:
@@ -595,16 +595,16 @@ class CudaBackend:
                 self._workspaces[(device, stream, 5)] = buf
         return buf
 
-    def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> tuple[Tensor, Tensor]:
+    def grad_norm(self, tensors: Sequence[Tensor], max_norm: float, clip: bool) -> tuple[Tensor, Tensor | None]:
         """(norm, factor) of all `tensors` together, on their device; with `clip` the tensors are
-        multiplied by the factor."""
-        marked = []
+        multiplied by the factor, which is not returned."""
+        marked = None
         if _grad_ready:
             stream = torch.cuda.current_stream(tensors[0].device)
             marked = _wait_grads(stream, tensors, keep=True)  # the step that follows may be on another stream
         rc, norm, factor = _tables.grad_norm(tensors, max_norm, clip, self._norm_scratch)
         check(rc)
-        if clip and marked:
+        if marked and clip:
             scaled = torch.cuda.Event()
             scaled.record(stream)
             _grad_ready.update(dict.fromkeys(marked, scaled))
