@@ -179,9 +179,10 @@ __device__ __forceinline__ int find_tensor(const S& start, int count, int chunk)
 // tensor are all aligned at one element (as in tensors packed one behind the other).
 constexpr unsigned char kNoHead = 255;
 
-// A step often follows a norm of the same gradients: it starts with the last of them, which are still in
-// L2. Norm and step of 218M bf16 weights with 8-bit moments take 416 us so, 422 in the order of the lists and with
-// ordinary accesses; 100M with float32 moments 121 and 127, 128 float32 filters 221 and 225.
+// A step often follows a norm of the same gradients: each launch starts with the last of its tensors, whose
+// gradients are still in L2 (a call with more tensors than a table holds launches its tables in the order of the
+// lists). Norm and step of 218M bf16 weights with 8-bit moments take 412 us so, 419 in the order of the lists and with
+// ordinary accesses; 100M bf16 weights with float32 moments 355 and 362, 128 float32 filters (47M) 225 and 229.
 __device__ __forceinline__ int from_the_end() { return (int)(gridDim.x - 1 - blockIdx.x); }
 
 struct AdamWConsts {
@@ -214,7 +215,9 @@ __device__ __forceinline__ bool read_factor(const float* grad_scale, float& f) {
 //   g' = g f;  m = b1 m + (1-b1) g';  v = b2 v + (1-b2) g'^2
 //   p  = p (1 - lr wd) - (lr/c1) m / (sqrt(v)/sqrt(c2) + eps)
 // in float32 registers, p rounded once when it is stored. With a master weight p is the master and
-// the parameter receives its rounded copy. Bound by HBM: 872M bf16 weights 2791 us, 6.9 TB/s.
+// the parameter receives its rounded copy. Bound by HBM: 872M bf16 weights 2791 us, 6.9 TB/s. Lists that are never
+// aligned together (packed parameters with moments of their own, say) go element by element: 100M weights 496 us
+// with bf16 and 472 with float32 parameters (4.4 and 5.9 TB/s), where aligned ones take 322 and 407.
 // ---------------------------------------------------------------------------
 template <int CAP>
 struct AdamW32Args {
@@ -441,8 +444,9 @@ __device__ __forceinline__ void both_factors(float m_amax, float v_amax, int lan
 }
 
 // 32 random bits for the four elements 4 * word .. 4 * word + 3; element j takes the low 20 bits of
-// the word turned right by 8 j. The multipliers are the fractional parts of the golden ratio and of
-// the square roots of 2 and 3.
+// the word turned right by 8 j. The multipliers are the prime 0x9E3779B1, which lies near the fractional part of
+// the golden ratio, and the fractional parts of the square roots of 2 and 3, in 32 bits; in the key those of the
+// square roots of 5 (made odd) and 3.
 __device__ __forceinline__ uint32_t random_word(uint32_t word, uint32_t key) {
   uint32_t h = word * 0x9E3779B1u + key;
   h = (h ^ (h >> 16)) * 0x6A09E667u;
@@ -608,7 +612,9 @@ constexpr int kShared8 = kWarps * kStages8 * Stage8<P, G, MASTER>::kBytes;
 // written once per task, lane k's for block k.
 // 436M bf16 weights: 655 us, 6.7 TB/s (1592 with plain loads, 1039 with the next block's loads in
 // registers); under the power cap, at 1.58 GHz, 755 us: 41 instructions an element keep the ALU pipe busy.
-// Lists that are not aligned go element by element (ragged_block8), at 3.1 to 4.1 TB/s.
+// Lists that are not aligned (8 parameters, 8 gradients and 8 masters each on a boundary of their size, 32 bytes
+// with float32) go element by element (ragged_block8): 100M weights 306 us with bf16 parameters and 405 with
+// float32, 3.3 and 4.0 TB/s, where aligned ones take 156 and 246.
 template <typename P, typename G, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm8)
 adamw8_kernel(const __grid_constant__ AdamW8Args<CAP> a) {
@@ -694,7 +700,9 @@ adamw8_kernel(const __grid_constant__ AdamW8Args<CAP> a) {
 
 // ---------------------------------------------------------------------------
 // Conversion of moments: 32-bit (or 16-bit) values <-> codes and scales. Bound by HBM: 218M values from float32
-// 155 us (7.05 TB/s), to bf16 98 us (6.7 TB/s).
+// 155 us (7.05 TB/s), to bf16 98 us (6.7 TB/s). Where values (by 8) or codes are not aligned, elements go one by one: 100M
+// values from float32 101 to 109 us (75 aligned), from bf16 107 to 115 (55); back, where values and codes are never aligned
+// together, to float32 164 us (77) and to bf16 151 (48).
 // ---------------------------------------------------------------------------
 constexpr int kBlocksPerWarp = 4;
 constexpr int kBlocksPerChunk = kWarps * kBlocksPerWarp;
@@ -1217,7 +1225,9 @@ int adamw8_launch(const AdamWCall& c, const AdamWConsts& consts, cudaStream_t st
 // Tensors per launch. Up to 32764 bytes of arguments hold several hundred, but handing them over takes the
 // host about 1 us for 6 KB: calls with fewer tensors take a smaller table. A call on 128 tensors of 768 elements
 // takes 14.3 us (AdamW), 12.8 (norm) and 15.7 (clipping) with the table for 160, and 17.8, 15.1 and 20.0 with the
-// largest one. A fourth size between 160 and the largest has not been built: 300 tensors take 108 ns each in both.
+// largest one; from 160 to 161 tensors it gets 2, 2 and 3.5 us longer. With 320 in the place of 160, 161 / 200 / 300
+// tensors took 0.6 / 3.3 / 1.6 us less (AdamW), 1.5 / 1.2 / 0.2 (norm) and 1.3 / 2.8 / 2.0 (clipping), and 90 and 150
+// tensors 0.4 to 7 us more.
 constexpr int kCapFew = 64, kCapSome = 160, kCapAdamW32 = 512, kCapAdamW8 = 384, kCapConvert = 512, kCapNorm = 1024;
 
 // f(std::integral_constant<int, CAP>) with the table that fits `count` tensors.
