@@ -92,6 +92,8 @@ def load_consolidated_state_dict(optimizer, state) -> None:
         wanted, kind = ("momentum", "Muon") if _is_muon_group(optimizer, group) else ("adam", "Adam")
         if wanted not in entry:
             raise ValueError(f"the checkpoint holds no {kind} state of a group that {type(optimizer).__name__} needs it for")
+        if ("state_bits" in entry["hyper"]) != isinstance(optimizer, AdamW):
+            raise ValueError(f"the checkpoint's groups do not hold the options of {type(optimizer).__name__}")
         params = group["params"]
         if [tuple(p.shape) for p in params] != [tuple(s) for s in entry["shapes"]]:
             raise ValueError("checkpoint and optimizer disagree on the parameter shapes of a group")

@@ -574,3 +574,20 @@ def test_an_extension_that_does_not_load_says_what_to_do(tmp_path):
         out = subprocess.run([sys.executable, "-c", "import muon_b200"], cwd=tmp_path, capture_output=True, text=True,
                              env={**os.environ, "PYTHONPATH": str(tmp_path)})
         assert out.returncode != 0 and "python muon_b200/build.py" in out.stderr and "_tables.so" in out.stderr
+
+
+def test_consolidated_checkpoints_of_the_auxiliary_adam_and_of_adamw_are_not_mixed(backend):
+    """Their groups hold different options, and their states different kinds of moments."""
+    import muon_b200 as mb
+    params = _params(6)[:2]
+    _give_grads(params, 1)
+    aux, adamw = mb.SingleDeviceMuonWithAuxAdam([dict(params=params, use_muon=False)]), mb.AdamW(params)
+    aux.step()
+    adamw.step()
+    for target, source in ((aux, adamw), (adamw, aux)):
+        before = [dict(g) for g in target.param_groups]
+        with pytest.raises(ValueError, match="options of"):
+            mb.load_consolidated_state_dict(target, mb.consolidated_state_dict(source))
+        assert [dict(g) for g in target.param_groups] == before
+        assert all(target.state[p]["step"] == 1 for p in params)
+        target.load_state_dict(target.state_dict())
